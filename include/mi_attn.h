@@ -213,8 +213,8 @@ void *mi_batch_stream(mi_batch *batch);
  * once and replay them. mi_batch_begin_capture opens a batch whose kernels
  * are recorded into a HIP graph (stream capture, relaxed mode) instead of
  * running. Only enqueueing calls belong in it (attention, copy_into_cache,
- * qk_norm_rope_cache(_value), rms_norm, rope, matmul, mi_batch_empty); no
- * upload, download or wait.
+ * qk_norm_rope_cache(_value), the packed and paged calls, rms_norm, rope, matmul,
+ * mi_batch_empty); no upload, download or wait.
  * mi_batch_end_capture consumes the batch and returns the graph, which keeps
  * the batch's scratch arena (so tensors leased during capture stay valid and
  * every replay writes the same addresses). Each replay reads and writes the
@@ -236,7 +236,8 @@ mi_status mi_context_synchronize(mi_context *ctx);
  * bound to its dispatch (hipExtLaunchKernelGGL), and its execution time is
  * reported per launch after wait. Names tell the kernels apart ("attn_rows",
  * "attn_decode", "attn_tiled", "attn_prefill", "attn_decode_stream"; the decode
- * step "attn_decode_step" or "attn_decode_step_mfma"; matmul "matvec",
+ * step "attn_decode_step" or "attn_decode_step_mfma"; the packed and paged calls
+ * "attn_packed", "attn_paged", "attn_decode_paged" and "qk_norm_rope_paged"; matmul "matvec",
  * "stream_matmul", "skinny_gemm", "gemm_tile" or the library's "gemm"), and
  * a merge launch is a record of its own ("attn_merge", "attn_tiled_merge",
  * "attn_decode_stream_merge"). */
@@ -398,6 +399,83 @@ mi_status mi_decode_step_attention(mi_batch *batch, const mi_tensor *q,
                                    const mi_qk_norm_rope_cache_config *qk_config,
                                    const mi_attention_config *config,
                                    const mi_tensor *out);
+
+/* --------------------------------------- packed rows, paged KV cache -- */
+
+/* Serving many sequences in one call. No counterpart in the reference (one
+ * sequence, one contiguous cache). Shared by the four calls below:
+ *  - Packed rows: a step's new tokens of all sequences, sequence after sequence,
+ *    as the rows of [N, H, D] tensors. row_starts, device u32 [B + 1]: sequence b
+ *    has the rows row_starts[b] to row_starts[b + 1] - 1 (none where they are
+ *    equal). Rows of no sequence (before the first, behind the last) are left as
+ *    they are in every output.
+ *  - Paged cache: key_pages / value_pages [P, S, Hkv, D], any strides with unit
+ *    innermost stride (storage [P, Hkv, S, D] keeps a head's keys together), S a
+ *    power of two of at least 16. block_table, device u32 [B, M] (any row
+ *    stride): position p of sequence b is in page block_table[b, p / S] at
+ *    p % S. An id of P or more names no page: no row sees its keys, and a row
+ *    that would be stored there is not. Sequences may share pages that they only
+ *    read; which of two rows written to one slot stays is not defined.
+ *  - lengths, device u32 [B]: keys of each sequence with the step's rows
+ *    appended (values above M * S are clamped to M * S). Row i of sequence b's n
+ *    rows has position lengths[b] - n + i, and sees keys 0 to that (all of them
+ *    where config->causal is 0). A row that sees no key, as of a sequence of
+ *    length 0, gets NaN (0/0); keys that a row does not see do not reach its
+ *    result, whatever they hold.
+ *  - head_dim 32, 64, 128 or 256, any group of query heads; bases and outer
+ *    strides of f16 tensors multiples of 16 bytes, position strides of keys and
+ *    values not negative. config->query_offset (and the transform's offset) are
+ *    ignored. Nothing is launched for N = 0 or B = 0.
+ *  - Tables, lengths and row offsets are read when the call runs on the GPU: a
+ *    captured call reads what they hold at each replay. Outputs must not overlap
+ *    inputs, except the transform's q_out, which may be q itself. */
+
+/* qk_norm_rope_cache_value for packed rows into pages: per-head RMSNorm with
+ * q_weight / k_weight [D] (both null: none), RoPE at each row's position, Q to
+ * q_out [N, Hq, D], K and the value rows [N, Hkv, D] into their pages. The angles
+ * are exact to f32 at any position (mi_rope computes them in f32). row_starts may
+ * be null: one row per sequence (N = B). A row without a position (more rows than
+ * lengths[b]) is not stored, and its q_out is left as it was. */
+mi_status mi_qk_norm_rope_paged(mi_batch *batch, const mi_tensor *q,
+                                const mi_tensor *k, const mi_tensor *value,
+                                const mi_tensor *q_weight,
+                                const mi_tensor *k_weight,
+                                const mi_tensor *key_pages,
+                                const mi_tensor *value_pages,
+                                const mi_tensor *block_table,
+                                const mi_tensor *lengths,
+                                const mi_tensor *row_starts,
+                                const mi_qk_norm_rope_cache_config *config,
+                                const mi_tensor *q_out);
+
+/* mi_attention_decode_batched over pages: one query row per sequence, q and
+ * out [B, Hq, D]. */
+mi_status mi_attention_decode_paged(mi_batch *batch, const mi_tensor *q,
+                                    const mi_tensor *key_pages,
+                                    const mi_tensor *value_pages,
+                                    const mi_tensor *block_table,
+                                    const mi_tensor *lengths,
+                                    const mi_attention_config *config,
+                                    const mi_tensor *out);
+
+/* Whole prompts: q and out [N, Hq, D] over the sequences' own rows of k and v
+ * [N, Hkv, D]. */
+mi_status mi_attention_packed(mi_batch *batch, const mi_tensor *q,
+                              const mi_tensor *k, const mi_tensor *v,
+                              const mi_tensor *row_starts,
+                              const mi_attention_config *config,
+                              const mi_tensor *out);
+
+/* Prompts, chunks and turns over the cache: q and out [N, Hq, D], keys and
+ * values in the sequences' pages (the step's own rows appended before). */
+mi_status mi_attention_paged(mi_batch *batch, const mi_tensor *q,
+                             const mi_tensor *key_pages,
+                             const mi_tensor *value_pages,
+                             const mi_tensor *block_table,
+                             const mi_tensor *lengths,
+                             const mi_tensor *row_starts,
+                             const mi_attention_config *config,
+                             const mi_tensor *out);
 
 /* ------------------------------------------------ attention neighbours -- */
 

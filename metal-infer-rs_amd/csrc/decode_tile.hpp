@@ -23,10 +23,12 @@ __device__ __forceinline__ int decode_slot_key(int r) {
 }
 // XOR applied to the 32-byte column pair of V row r: the 16 rows of one
 // transposed read then fall on 8 distinct bank groups (D = 64: rows are half a
-// bank row, so their parity already picks one of two halves).
+// bank row, so their parity already picks one of two halves; D = 32: a quarter).
 template <int D>
 __device__ __forceinline__ int decode_v_swizzle(int r) {
-  return D == 128 ? ((r & 3) | (((r >> 3) & 1) << 2)) : (((r >> 1) & 1) | (((r >> 3) & 1) << 1));
+  return D >= 128  ? ((r & 3) | (((r >> 3) & 1) << 2))
+         : D == 64 ? (((r >> 1) & 1) | (((r >> 3) & 1) << 1))
+                   : ((r >> 3) & 1);
 }
 
 // Whether any of a wave's `bytes` of LDS at `lds` (a multiple of 1 KB) is an f16

@@ -327,6 +327,76 @@ constexpr uint64_t tiled_partial_floats(uint64_t splits, uint64_t row_tiles, uin
   return splits * row_tiles * kv_heads * 4 * 64 * (head_dim / 2 + 2);
 }
 hipError_t launch_tiled(const PrefillParams &p, uint32_t head_dim, TiledPhase phase, const Launch &l);
+// Keys and values in pages: [pages, 2^page_shift, Hkv, D] views, and of each sequence
+// the pages it has (table [B, table_width], rows table_seq words apart) and its length.
+// A page id past the last page names no page: its keys are seen by no row. Within a
+// page the position stride is not negative and the page spans less than 2 GiB.
+struct PagedKv {
+  const uint16_t *k;
+  int64_t k_page, k_pos, k_head;
+  const uint16_t *v;
+  int64_t v_page, v_pos, v_head;
+  const uint32_t *table;
+  int64_t table_seq;
+  const uint32_t *lengths;
+  uint32_t pages, page_shift, table_width;
+};
+constexpr uint32_t kPagedMinShift = 4;  // pages of at least 16 positions
+
+// QK-norm (weights not null) and RoPE of packed rows, K and V into their pages. Row r
+// of sequence b (row_starts[b] <= r < row_starts[b + 1]; null: sequence b is row b) has
+// position lengths[b] - row_starts[b + 1] + r.
+struct PagedAppendParams {
+  const uint16_t *q;
+  int64_t q_tok, q_head;
+  const uint16_t *k;
+  int64_t k_tok, k_head;
+  const uint16_t *v;
+  int64_t v_tok, v_head;
+  const uint16_t *q_weight, *k_weight;
+  uint16_t *q_out;
+  int64_t qo_tok, qo_head;
+  PagedKv kv;
+  uint16_t *key_pages, *value_pages;  // kv.k and kv.v, to write
+  const uint32_t *row_starts;
+  uint32_t rows, batch, q_heads, kv_heads;
+  float epsilon;
+  double log2_theta;
+};
+hipError_t launch_paged_append(const PagedAppendParams &p, uint32_t head_dim, const Launch &l);
+
+// One query row per sequence over its pages. Q and O are [B, Hq, D].
+struct PagedDecodeParams {
+  const uint16_t *q;
+  int64_t q_seq, q_head;
+  uint16_t *out;
+  int64_t o_seq, o_head;
+  PagedKv kv;
+  uint32_t batch, q_heads, kv_heads, group;
+  uint32_t head_chunks, chunk;  // a KV head's query heads in chunks of at most kDecodeRows
+  float scale_log2;
+};
+hipError_t launch_paged_decode(const PagedDecodeParams &p, uint32_t head_dim, const Launch &l);
+
+// Packed query rows [N, Hq, D] of `batch` sequences over their own packed rows of K and
+// V (kv.table null: kv.k_pos and v_pos are row strides), or over their pages.
+struct PackedParams {
+  const uint16_t *q;
+  int64_t q_tok, q_head;
+  uint16_t *out;
+  int64_t o_tok, o_head;
+  PagedKv kv;
+  const uint32_t *row_starts;
+  uint32_t rows, batch, q_heads, kv_heads, group, causal;
+  uint32_t row_tiles;  // most row tiles of a KV head (host bound)
+  float scale_log2;
+};
+hipError_t launch_packed(const PackedParams &p, uint32_t head_dim, const Launch &l);
+// Most row tiles of a KV head: every sequence may have a partial one.
+uint64_t packed_row_tiles(uint64_t rows, uint32_t batch, uint32_t group);
+// Head dimensions of the kernels over packed rows and pages.
+constexpr bool paged_head_dim(uint64_t d) { return d == 32 || d == 64 || d == 128 || d == 256; }
+
 // Capacity of a context's split-K arrival counters (u32 words: units of a
 // fused rows plan, row tiles x KV heads of a split prefill grid, each at
 // counter_stride words).

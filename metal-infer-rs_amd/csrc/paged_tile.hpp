@@ -1,0 +1,54 @@
+// What the kernels over packed rows and the paged KV cache share: which sequence a
+// row belongs to, and where the rows that no sequence has are read from.
+#pragma once
+
+#include "device_common.hpp"
+#include "kernels.hpp"
+
+namespace mi {
+namespace dev {
+
+// A key row of zeros (the largest head_dim). Rows of a tile past its last key, and
+// those of a page that is not there, are read from here: a masked weight is 0, and 0
+// times what a recycled page holds (infinities, NaN) would be NaN in the products.
+static __device__ __attribute__((aligned(512))) uint16_t zero_row[256];
+
+// Sequence `b`'s packed rows [begin, end) of the call's `rows`, whatever the
+// offsets hold (they are device data: out-of-order ones make an empty sequence).
+struct RowRange {
+  uint32_t begin, end;
+};
+__device__ __forceinline__ RowRange sequence_rows(const uint32_t *row_starts, uint32_t b, uint32_t rows) {
+  if (row_starts == nullptr) return {min(b, rows), min(b + 1, rows)};
+  const uint32_t end = min(row_starts[b + 1], rows);
+  return {min(row_starts[b], end), end};
+}
+
+// The last sequence that starts at or before `row` (uniform over the wave), which is
+// the one that holds it if any does: sequences without rows start where the next one
+// does.
+__device__ __forceinline__ uint32_t sequence_of_row(const uint32_t *row_starts, uint32_t batch, uint32_t row,
+                                                    int lane) {
+  if (row_starts == nullptr) return min(row, batch - 1);
+  uint32_t count = 0;
+  for (uint32_t c0 = 1; c0 < batch; c0 += 64) {
+    const uint32_t b = c0 + lane;
+    count += (uint32_t)__popcll(__ballot(b < batch && row_starts[b] <= row));
+  }
+  return count;
+}
+
+// Keys of sequence `b`: its length, within what its table row can name.
+__device__ __forceinline__ uint32_t paged_length(const kernels::PagedKv &kv, uint32_t b) {
+  return min(kv.lengths[b], kv.table_width << kv.page_shift);
+}
+
+// s_waitcnt vmcnt(N), the other counters left at their maxima.
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  static_assert(N >= 0 && N < 64, "vmcnt is six bits");
+  __builtin_amdgcn_s_waitcnt(kWaitVmcnt0 | (N & 15) | ((N >> 4) << 14));
+}
+
+}  // namespace dev
+}  // namespace mi

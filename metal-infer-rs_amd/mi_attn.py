@@ -153,6 +153,13 @@ def _load() -> ctypes.CDLL:
         "mi_decode_step_attention": (ctypes.c_int, [ctypes.c_void_p, T, T, T, T, T, T, T,
                                                     _P(QkNormRopeCacheConfig),
                                                     _P(AttentionConfig), T]),
+        "mi_qk_norm_rope_paged": (ctypes.c_int, [ctypes.c_void_p] + [T] * 10 +
+                                  [_P(QkNormRopeCacheConfig), T]),
+        "mi_attention_decode_paged": (ctypes.c_int, [ctypes.c_void_p, T, T, T, T, T,
+                                                     _P(AttentionConfig), T]),
+        "mi_attention_packed": (ctypes.c_int, [ctypes.c_void_p, T, T, T, T, _P(AttentionConfig), T]),
+        "mi_attention_paged": (ctypes.c_int, [ctypes.c_void_p, T, T, T, T, T, T,
+                                              _P(AttentionConfig), T]),
         "mi_rms_norm": (ctypes.c_int, [ctypes.c_void_p, T, T, ctypes.c_float, T]),
         "mi_rope": (ctypes.c_int, [ctypes.c_void_p, T, ctypes.c_uint64, ctypes.c_float, T]),
         "mi_matmul": (ctypes.c_int, [ctypes.c_void_p, T, T, T]),
@@ -189,6 +196,11 @@ def header_symbols() -> list[str]:
 def _check(status: int) -> None:
     if status != 0:
         raise MiError(status, (lib().mi_last_error() or b"").decode())
+
+
+def _ref(tensor):
+    """A tensor's descriptor for the C call, or null for an optional one that is None."""
+    return None if tensor is None else ctypes.byref(tensor.desc)
 
 
 def _shape_array(shape):
@@ -544,6 +556,49 @@ class Batch:
             self.handle, ctypes.byref(q.desc), ctypes.byref(k.desc), ctypes.byref(value.desc),
             ctypes.byref(q_weight.desc), ctypes.byref(k_weight.desc), ctypes.byref(key_cache.desc),
             ctypes.byref(value_cache.desc), ctypes.byref(qk_config), ctypes.byref(config),
+            ctypes.byref(out.desc)))
+        return out
+
+    def qk_norm_rope_paged(self, q, k, value, q_weight, k_weight, key_pages, value_pages,
+                           block_table, lengths, config: QkNormRopeCacheConfig, row_starts=None,
+                           out=None) -> Tensor:
+        """qk_norm_rope_cache_value of packed rows [N, H, D] into the pages of their
+        sequences; weights None: no norm, row_starts None: one row per sequence."""
+        out = self._out(q.shape, out)
+        _check(lib().mi_qk_norm_rope_paged(
+            self.handle, ctypes.byref(q.desc), ctypes.byref(k.desc), ctypes.byref(value.desc),
+            _ref(q_weight), _ref(k_weight), ctypes.byref(key_pages.desc),
+            ctypes.byref(value_pages.desc), ctypes.byref(block_table.desc),
+            ctypes.byref(lengths.desc), _ref(row_starts), ctypes.byref(config),
+            ctypes.byref(out.desc)))
+        return out
+
+    def attention_decode_paged(self, q, key_pages, value_pages, block_table, lengths,
+                               config: AttentionConfig, out=None) -> Tensor:
+        """Attention of one query row per sequence [B, Hq, D] over its pages."""
+        out = self._out(q.shape, out)
+        _check(lib().mi_attention_decode_paged(
+            self.handle, ctypes.byref(q.desc), ctypes.byref(key_pages.desc),
+            ctypes.byref(value_pages.desc), ctypes.byref(block_table.desc),
+            ctypes.byref(lengths.desc), ctypes.byref(config), ctypes.byref(out.desc)))
+        return out
+
+    def attention_packed(self, q, k, v, row_starts, config: AttentionConfig, out=None) -> Tensor:
+        """Attention of packed rows [N, H, D] within their sequences."""
+        out = self._out(q.shape, out)
+        _check(lib().mi_attention_packed(
+            self.handle, ctypes.byref(q.desc), ctypes.byref(k.desc), ctypes.byref(v.desc),
+            ctypes.byref(row_starts.desc), ctypes.byref(config), ctypes.byref(out.desc)))
+        return out
+
+    def attention_paged(self, q, key_pages, value_pages, block_table, lengths, row_starts,
+                        config: AttentionConfig, out=None) -> Tensor:
+        """Attention of packed rows [N, Hq, D] over the pages of their sequences."""
+        out = self._out(q.shape, out)
+        _check(lib().mi_attention_paged(
+            self.handle, ctypes.byref(q.desc), ctypes.byref(key_pages.desc),
+            ctypes.byref(value_pages.desc), ctypes.byref(block_table.desc),
+            ctypes.byref(lengths.desc), ctypes.byref(row_starts.desc), ctypes.byref(config),
             ctypes.byref(out.desc)))
         return out
 

@@ -228,6 +228,29 @@ extern "C" {
                                     config: *const mi_attention_config, out: *const mi_tensor)
         -> mi_status;
 
+    // packed rows, paged KV cache
+    pub fn mi_qk_norm_rope_paged(batch: *mut mi_batch, q: *const mi_tensor, k: *const mi_tensor,
+                                 value: *const mi_tensor, q_weight: *const mi_tensor,
+                                 k_weight: *const mi_tensor, key_pages: *const mi_tensor,
+                                 value_pages: *const mi_tensor, block_table: *const mi_tensor,
+                                 lengths: *const mi_tensor, row_starts: *const mi_tensor,
+                                 config: *const mi_qk_norm_rope_cache_config,
+                                 q_out: *const mi_tensor) -> mi_status;
+    pub fn mi_attention_decode_paged(batch: *mut mi_batch, q: *const mi_tensor,
+                                     key_pages: *const mi_tensor, value_pages: *const mi_tensor,
+                                     block_table: *const mi_tensor, lengths: *const mi_tensor,
+                                     config: *const mi_attention_config, out: *const mi_tensor)
+        -> mi_status;
+    pub fn mi_attention_packed(batch: *mut mi_batch, q: *const mi_tensor, k: *const mi_tensor,
+                               v: *const mi_tensor, row_starts: *const mi_tensor,
+                               config: *const mi_attention_config, out: *const mi_tensor)
+        -> mi_status;
+    pub fn mi_attention_paged(batch: *mut mi_batch, q: *const mi_tensor,
+                              key_pages: *const mi_tensor, value_pages: *const mi_tensor,
+                              block_table: *const mi_tensor, lengths: *const mi_tensor,
+                              row_starts: *const mi_tensor, config: *const mi_attention_config,
+                              out: *const mi_tensor) -> mi_status;
+
     // attention neighbours
     pub fn mi_rms_norm(batch: *mut mi_batch, input: *const mi_tensor, weight: *const mi_tensor,
                        epsilon: f32, out: *const mi_tensor) -> mi_status;

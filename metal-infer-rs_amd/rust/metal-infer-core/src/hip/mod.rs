@@ -690,6 +690,72 @@ impl<'context> CommandBatch<'context> {
         Ok(out)
     }
 
+    /// qk_norm_rope_cache_value of packed rows [N, H, D] into the pages of
+    /// their sequences (no reference counterpart): pages [P, S, Hkv, D],
+    /// block_table u32 [B, M], lengths u32 [B], row_starts u32 [B + 1] (None:
+    /// one row per sequence). Both weights None: no norm.
+    #[allow(clippy::too_many_arguments)]
+    pub fn qk_norm_rope_paged(&mut self, query: &Tensor, key: &Tensor, value: &Tensor,
+                              query_weight: Option<&Tensor>, key_weight: Option<&Tensor>,
+                              key_pages: &Tensor, value_pages: &Tensor, block_table: &Tensor,
+                              lengths: &Tensor, row_starts: Option<&Tensor>,
+                              config: QkNormRopeCacheConfig)
+        -> Result<Tensor, CoreError> {
+        let cfg = qk_config(config)?;
+        let out = self.empty(query.shape(), DType::F16)?;
+        let raw = |t: Option<&Tensor>| -> *const mi_tensor {
+            t.map_or(std::ptr::null(), |t| &t.desc)
+        };
+        check(unsafe {
+            mi_qk_norm_rope_paged(self.raw, &query.desc, &key.desc, &value.desc,
+                                  raw(query_weight), raw(key_weight), &key_pages.desc,
+                                  &value_pages.desc, &block_table.desc, &lengths.desc,
+                                  raw(row_starts), &cfg, &out.desc)
+        })?;
+        Ok(out)
+    }
+
+    /// Attention of one query row per sequence [B, Hq, D] over its pages.
+    pub fn attention_decode_paged(&mut self, query: &Tensor, key_pages: &Tensor,
+                                  value_pages: &Tensor, block_table: &Tensor, lengths: &Tensor,
+                                  config: AttentionConfig) -> Result<Tensor, CoreError> {
+        let cfg = attention_config(config)?;
+        let out = self.empty(query.shape(), DType::F16)?;
+        check(unsafe {
+            mi_attention_decode_paged(self.raw, &query.desc, &key_pages.desc, &value_pages.desc,
+                                      &block_table.desc, &lengths.desc, &cfg, &out.desc)
+        })?;
+        Ok(out)
+    }
+
+    /// Attention of packed rows [N, H, D] within their sequences.
+    pub fn attention_packed(&mut self, query: &Tensor, key: &Tensor, value: &Tensor,
+                            row_starts: &Tensor, config: AttentionConfig)
+        -> Result<Tensor, CoreError> {
+        let cfg = attention_config(config)?;
+        let out = self.empty(query.shape(), DType::F16)?;
+        check(unsafe {
+            mi_attention_packed(self.raw, &query.desc, &key.desc, &value.desc, &row_starts.desc,
+                                &cfg, &out.desc)
+        })?;
+        Ok(out)
+    }
+
+    /// Attention of packed rows [N, Hq, D] over the pages of their sequences.
+    #[allow(clippy::too_many_arguments)]
+    pub fn attention_paged(&mut self, query: &Tensor, key_pages: &Tensor, value_pages: &Tensor,
+                           block_table: &Tensor, lengths: &Tensor, row_starts: &Tensor,
+                           config: AttentionConfig) -> Result<Tensor, CoreError> {
+        let cfg = attention_config(config)?;
+        let out = self.empty(query.shape(), DType::F16)?;
+        check(unsafe {
+            mi_attention_paged(self.raw, &query.desc, &key_pages.desc, &value_pages.desc,
+                               &block_table.desc, &lengths.desc, &row_starts.desc, &cfg,
+                               &out.desc)
+        })?;
+        Ok(out)
+    }
+
     /// ops.rs:722-755.
     pub fn rms_norm(&mut self, input: &Tensor, weight: &Tensor, epsilon: f32)
         -> Result<Tensor, CoreError> {
