@@ -13,6 +13,7 @@ namespace mi {
 namespace {
 
 constexpr uint64_t kRows31 = 1ull << 31;
+constexpr uint64_t kDecodeTileKeys = 32;  // keys of the decode kernel's tile
 
 mi_status check_batch(const mi_batch *batch) {
   if (batch == nullptr) return fail(MI_ERR_INVALID_ARGUMENT, "null batch");
@@ -143,12 +144,36 @@ mi_status decode_paged(mi_batch *batch, const mi_tensor *q, const mi_tensor *key
   p.head_chunks = (p.group + kernels::kDecodeRows - 1) / kernels::kDecodeRows;
   p.chunk = (p.group + p.head_chunks - 1) / p.head_chunks;
   p.scale_log2 = scale_log2(config->head_dim);
-  if ((uint64_t)p.batch * p.kv_heads * p.head_chunks >= kRows31)
+  // As many sequences a launch as its limits take (512 of 8 KV heads), which fill the
+  // chip by themselves.
+  const uint64_t upb = (uint64_t)p.kv_heads * p.head_chunks;
+  const uint64_t most_tiles = ((uint64_t)p.kv.table_width << p.kv.page_shift) / kDecodeTileKeys + 1;
+  if (upb > kernels::kPagedMaxUnits || upb * most_tiles >= kRows31)
     return fail(MI_ERR_SHAPE, "attention grid exceeds the launch limits");
   if ((st = check_batch(batch)) != MI_OK || q->shape[0] == 0) return st;
-  return launch(batch, "attn_decode_paged", [&](const kernels::Launch &s) {
-    return kernels::launch_paged_decode(p, config->head_dim, s);
-  });
+  Context *ctx = batch->ctx;
+  const uint32_t step = (uint32_t)std::min<uint64_t>(
+      {kernels::kPagedMaxBatch, kernels::kPagedMaxUnits / upb, (kRows31 - 1) / (upb * most_tiles), p.batch});
+  p.workgroups = kernels::paged_decode_workgroups(ctx->compute_units, config->head_dim);
+  p.counters = ctx->split_counters;
+  p.counter_stride = kernels::counter_stride(step * upb, ctx->split_counter_count);
+  void *scratch = nullptr;
+  const uint64_t floats =
+      kernels::paged_decode_partial_floats(step * upb, p.workgroups, p.chunk, config->head_dim);
+  if ((st = scratch_alloc(batch, floats * sizeof(float), &scratch)) != MI_OK) return st;
+  p.partial = static_cast<float *>(scratch);
+  for (uint32_t first = 0; first < (uint32_t)q->shape[0] && st == MI_OK; first += step) {
+    kernels::PagedDecodeParams part = p;
+    part.batch = std::min(step, p.batch - first);
+    part.q += first * p.q_seq, part.out += first * p.o_seq;
+    part.kv.table += first * p.kv.table_seq, part.kv.lengths += first;
+    st = launch(batch, "attn_decode_paged", [&](const kernels::Launch &s) {
+      return kernels::launch_paged_decode(part, config->head_dim, s);
+    });
+  }
+  // In-order execution makes the range reusable by later work of the batch.
+  scratch_free(ctx, scratch);
+  return st;
 }
 
 // Packed rows over their own K and V rows (block_table null) or over pages.
