@@ -366,14 +366,14 @@ struct PagedAppendParams {
 hipError_t launch_paged_append(const PagedAppendParams &p, uint32_t head_dim, const Launch &l);
 
 // One query row per sequence over its pages. Q and O are [B, Hq, D]. A unit is
-// (sequence, KV head, head chunk); a unit that several workgroups share needs a counter
-// (zero between kernels, counter_stride words apart) and one partial of chunk *
-// (head_dim + 2) floats per piece: paged_decode_partial_floats in all. At most
+// (sequence, KV head, head chunk); a unit that several waves share needs a counter
+// (zero between kernels, counter_stride words apart) and partials of chunk *
+// (head_dim + 2) floats: paged_decode_partial_floats in all. At most
 // kPagedMaxBatch sequences, kPagedMaxUnits units and 2^31 (unit, 32-key tile)s a launch.
-constexpr uint32_t kPagedMaxBatch = 1024, kPagedMaxUnits = 4096;
+constexpr uint32_t kPagedMaxBatch = 512, kPagedMaxUnits = 4096, kPagedWaves = 4;
 constexpr uint64_t paged_decode_partial_floats(uint64_t units, uint64_t workgroups, uint32_t chunk,
                                                uint32_t head_dim) {
-  return (units + workgroups) * chunk * (head_dim + 2);
+  return (units + workgroups * kPagedWaves) * chunk * (head_dim + 2);
 }
 uint32_t paged_decode_workgroups(uint32_t compute_units, uint32_t head_dim);
 struct PagedDecodeParams {
@@ -388,6 +388,7 @@ struct PagedDecodeParams {
   float *partial;
   uint32_t *counters;
   uint32_t counter_stride, workgroups;
+  uint32_t *step_counters;  // one per workgroup
 };
 hipError_t launch_paged_decode(const PagedDecodeParams &p, uint32_t head_dim, const Launch &l);
 

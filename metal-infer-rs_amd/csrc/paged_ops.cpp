@@ -155,8 +155,11 @@ mi_status decode_paged(mi_batch *batch, const mi_tensor *q, const mi_tensor *key
   const uint32_t step = (uint32_t)std::min<uint64_t>(
       {kernels::kPagedMaxBatch, kernels::kPagedMaxUnits / upb, (kRows31 - 1) / (upb * most_tiles), p.batch});
   p.workgroups = kernels::paged_decode_workgroups(ctx->compute_units, config->head_dim);
-  p.counters = ctx->split_counters;
-  p.counter_stride = kernels::counter_stride(step * upb, ctx->split_counter_count);
+  if (p.workgroups + kernels::kPagedMaxUnits > ctx->split_counter_count)
+    return fail(MI_ERR_RESOURCE, "too few split counters");
+  p.step_counters = ctx->split_counters;
+  p.counters = ctx->split_counters + p.workgroups;
+  p.counter_stride = kernels::counter_stride(step * upb, ctx->split_counter_count - p.workgroups);
   void *scratch = nullptr;
   const uint64_t floats =
       kernels::paged_decode_partial_floats(step * upb, p.workgroups, p.chunk, config->head_dim);

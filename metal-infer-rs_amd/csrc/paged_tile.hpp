@@ -43,12 +43,25 @@ __device__ __forceinline__ uint32_t paged_length(const kernels::PagedKv &kv, uin
   return min(kv.lengths[b], kv.table_width << kv.page_shift);
 }
 
+// The parameters of a kernel of one parameter, read again: what is used only before and
+// after a loop then takes none of its scalar registers (the compiler would keep every
+// parameter from the first read to the last use, and spill).
+template <typename Params>
+__device__ __forceinline__ const Params __attribute__((address_space(4))) *params_again() {
+  auto at = (const Params __attribute__((address_space(4))) *)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  return at;
+}
+
 // s_waitcnt vmcnt(N), the other counters left at their maxima.
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
   static_assert(N >= 0 && N < 64, "vmcnt is six bits");
   __builtin_amdgcn_s_waitcnt(kWaitVmcnt0 | (N & 15) | ((N >> 4) << 14));
 }
+
+// s_waitcnt lgkmcnt(0): the wave's LDS accesses are done.
+__device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xC07F); }
 
 }  // namespace dev
 }  // namespace mi
