@@ -38,7 +38,8 @@ typedef float f4_t __attribute__((ext_vector_type(4)));
 constexpr uint32_t per_cu(uint32_t) { return 2; }
 // Fewest tiles of a workgroup's piece (one per wave) and of a wave's share.
 constexpr uint32_t kPiece = kWaves, kShare = 2;
-// Units from which each wave works by itself, and parts that are joined in one step.
+// Units from which each wave works by itself; more than twice kJoin pieces are joined in
+// steps of kJoin.
 constexpr uint32_t kManyUnits = 128, kJoin = 16;
 
 // Sum of x over the lanes up to this one (row shifts, then the rows' last lanes).
@@ -131,7 +132,7 @@ template <int D>
 __device__ __forceinline__ void join_parts(float *partial, size_t row_stride, uint32_t parts, uint32_t heads,
                                            float scale_log2, uint16_t *out, int64_t o_head, uint32_t first,
                                            uint32_t step, float *s_f, int lane) {
-  constexpr uint32_t ROW = D + 2, MOST = 32, KU = D == 32 ? 2 : D == 256 ? 4 : 4, PU = 16 / KU;
+  constexpr uint32_t ROW = D + 2, MOST = 32, KU = 2, PU = 8;
   constexpr uint32_t BLOCK = 64 * KU, HEADS = BLOCK / (D / 2), FROW = MOST + 2;
   static_assert(HEADS * FROW * 4 <= 2048 && BLOCK % (D / 2) == 0, "a block is of whole heads");
   const uint32_t pairs = heads * (D / 2);
@@ -523,7 +524,7 @@ __global__ __launch_bounds__(kWaves * 64, per_cu(D)) void attn_decode_paged_kern
   const size_t row_stride = (size_t)e->chunk * ROW;
   float *spare = reinterpret_cast<float *>(stage);
   // Its units' joins are the wave's own; in a workgroup's piece of a split unit, the last
-  // of the unit's pieces joins them all, or 16 of them, and the last of those steps the
+  // of the unit's pieces joins them all, or kJoin of them, and the last of those steps the
   // steps (256 pieces by one workgroup took 70 us).
   uint32_t n = together ? split : done, step = 0;
   for (uint32_t i = 0; i < n; ++i) {
@@ -532,7 +533,7 @@ __global__ __launch_bounds__(kWaves * 64, per_cu(D)) void attn_decode_paged_kern
     size_t apart = row_stride;
     uint16_t *out = rows_of(u, &heads);
     if (together) {
-      const uint32_t groups = u.pieces > kJoin ? (u.pieces + kJoin - 1) / kJoin : 1;
+      const uint32_t groups = u.pieces > 2 * kJoin ? (u.pieces + kJoin - 1) / kJoin : 1;
       uint32_t *counter = e->counters + (size_t)(u.b * upb + u.j) * e->counter_stride;
       if (groups > 1 && step == 0) {
         first = (w - u.slot) / kJoin * kJoin;
