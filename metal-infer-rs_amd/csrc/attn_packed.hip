@@ -13,6 +13,12 @@
 //    (ds_read_b64_tr_b16);
 //  - the next tile's direct global -> LDS loads are in flight while one is computed. A
 //    wave loads 16 (or 8) consecutive rows of a tile, so they lie in one page.
+//  - Order: the work per row tile is known on the device only. Every workgroup works out
+//    the same plan from the sequences' rows and lengths and takes the piece of its rank:
+//    tiles with more keys than a workgroup's even share are cut into pieces, which come
+//    first, then the whole tiles with most keys first. The pieces of a cut tile leave
+//    their max, sum and weighted values (f32), and the last of them to finish joins them
+//    in order.
 // Bound by the matrix instructions with the exponentials beside them for long prompts,
 // by the bytes of K and V for a few rows on a long cache.
 #include <type_traits>
@@ -31,11 +37,154 @@ constexpr int BM = kPrefillBlockM;  // rows per workgroup
 // Added to every weight's exponent, so that f16 holds weights down to 2^-32 of the
 // reference's (a long tail of them counts); it cancels against the row sum.
 constexpr float kBias = 8.0f;
+// Fewest key tiles of a piece of a cut row tile, and most pieces.
+constexpr uint32_t kLeastPiece = 4, kMostPieces = 16;
 constexpr int kReadAhead = 4;       // LDS operand reads in flight ahead of the MFMAs
 constexpr int kSchedMfma = 0x008, kSchedDsRead = 0x100;
 
-__device__ __forceinline__ uint32_t row_tiles_of(RowRange r, uint32_t group) {
-  return ((r.end - r.begin) * group + BM - 1) / BM;
+// A sequence as the plan sees it: its packed (token, head) rows, and the position of its
+// first row (negative: more rows than keys).
+struct Rows {
+  uint32_t rows;
+  int32_t first;
+};
+
+// Row tiles and their 64-key tiles.
+struct Tiles {
+  uint32_t group, causal;
+  __device__ __forceinline__ uint32_t count(Rows r) const { return (r.rows + BM - 1) / BM; }
+  // Keys that the last row of tile i sees.
+  __device__ __forceinline__ uint32_t keys(Rows r, uint32_t i) const {
+    const int32_t tokens = (int32_t)(r.rows / group);
+    const int32_t last = causal != 0 ? min(tokens - 1, (int32_t)(((i + 1) * BM - 1) / group)) : tokens - 1;
+    return (uint32_t)max(0, r.first + last + 1);
+  }
+  __device__ __forceinline__ uint32_t key_tiles(Rows r, uint32_t i) const { return (keys(r, i) + BN - 1) / BN; }
+  // The first row tile with at least x key tiles (the count of them if none has).
+  __device__ __forceinline__ uint32_t first_with(Rows r, uint32_t x) const {
+    const uint32_t all = count(r);
+    if (all == 0 || key_tiles(r, 0) >= x) return 0;
+    if (key_tiles(r, all - 1) < x) return all;
+    // Causal, x > 0: the tile of the first token that sees key (x - 1) BN.
+    return (uint32_t)((int32_t)((x - 1) * BN) - r.first) * group / BM;
+  }
+};
+
+// Sums and the like over the 64 lanes, to every lane.
+__device__ __forceinline__ uint32_t wave_sum(uint32_t x) { return last_lane(scan64(x)); }
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x = max(x, (uint32_t)__shfl_xor((int)x, d, 64));
+  return x;
+}
+
+// What the workgroup of a rank does: key tiles [begin, end) of a row tile, as piece
+// `piece` of `pieces`; `cut` numbers the tiles that are cut.
+struct Piece {
+  uint32_t b, tile, begin, end, piece, pieces, cut;
+};
+
+// The piece of `rank` (of one KV head), the same in every wave that asks. `share`: the
+// workgroups that the chip runs at once for one KV head.
+__device__ __forceinline__ bool plan_piece(const PackedParams &p, uint32_t rank, const Rows *s_rows, uint32_t *s_before, int lane,
+                           Piece *out) {
+  const Tiles t{p.group, p.causal};
+  auto rows_of = [&](uint32_t b) { return b < p.batch ? s_rows[b] : Rows{0, 0}; };
+  uint32_t all = 0, most = 0, work = 0;  // row tiles; key tiles of the longest; of all (about)
+  for (uint32_t c0 = 0; c0 < p.batch; c0 += 64) {
+    const Rows r = rows_of(c0 + lane);
+    const uint32_t n = t.count(r);
+    if (n == 0) continue;
+    const uint32_t lo = t.key_tiles(r, 0), hi = t.key_tiles(r, n - 1);
+    all += n;
+    most = max(most, hi);
+    work += n * (lo + hi + 1) / 2;
+  }
+  all = wave_sum(all), most = wave_max(most), work = wave_sum(work);
+  if (rank >= all + p.max_pieces) return false;
+  // Most key tiles of a piece: an even share (room for the pieces that do not fill up,
+  // half a piece per tile, where all of them fit the chip at once), at least kLeastPiece,
+  // and at most kMostPieces pieces a tile.
+  uint32_t cap = most;
+  if (most >= 2 * kLeastPiece && p.max_pieces != 0) {
+    const uint32_t slots = all < p.share ? p.share - all / 2 : p.share;
+    cap = max(max(kLeastPiece, (work + slots - 1) / slots), (most + kMostPieces - 1) / kMostPieces);
+  }
+  // The cut tiles: those of at least cap + 1 key tiles, sequence after sequence.
+  uint32_t cuts = 0, pieces = 0;
+  bool found = false;
+  for (;; cap *= 2) {
+    cuts = pieces = 0;
+    found = false;
+    if (cap >= most) break;
+    for (uint32_t c0 = 0; c0 < p.batch; c0 += 64) {
+      const Rows r = rows_of(c0 + lane);
+      const uint32_t x = scan64(t.count(r) - t.first_with(r, cap + 1));
+      if (c0 + lane < p.batch) s_before[c0 + lane + 1] = cuts + x;
+      cuts += last_lane(x);
+    }
+    if (lane == 0) s_before[0] = 0;
+    if (cuts > p.max_pieces) continue;
+    for (uint32_t k0 = 0; k0 < cuts; k0 += 64) {
+      const uint32_t k = k0 + lane;
+      uint32_t lo = 0;  // the last sequence with s_before[lo] <= k
+      for (uint32_t step = 512; step != 0; step >>= 1)
+        if (lo + step < p.batch && s_before[lo + step] <= k) lo += step;
+      const Rows r = rows_of(lo);
+      const uint32_t i = k < cuts ? t.first_with(r, cap + 1) + k - s_before[lo] : 0;
+      const uint32_t n = k < cuts ? t.key_tiles(r, i) : 0, s = (n + cap - 1) / cap;
+      const uint32_t x = scan64(s);
+      const uint64_t le = __ballot(pieces + x <= rank);
+      if (!found && le != ~0ull) {
+        const int at = __popcll(le);
+        const uint32_t s_at = (uint32_t)__builtin_amdgcn_readlane((int)s, at);
+        const uint32_t n_at = (uint32_t)__builtin_amdgcn_readlane((int)n, at);
+        const uint32_t z = rank - (pieces + (uint32_t)__builtin_amdgcn_readlane((int)x, at) - s_at);
+        *out = {(uint32_t)__builtin_amdgcn_readlane((int)lo, at), (uint32_t)__builtin_amdgcn_readlane((int)i, at),
+                z * n_at / s_at, (z + 1) * n_at / s_at, z, s_at, k0 + at};
+        found = true;
+      }
+      pieces += last_lane(x);
+    }
+    if (pieces <= p.max_pieces) break;
+  }
+  if (found) return true;
+  // The whole tiles, most key tiles first: the largest x of which more than rank tiles
+  // have at least x.
+  rank -= pieces;
+  if (rank >= all - cuts) return false;
+  auto at_least = [&](uint32_t x) -> uint32_t {
+    uint32_t n = 0;
+    for (uint32_t c0 = 0; c0 < p.batch; c0 += 64) {
+      const Rows r = rows_of(c0 + lane);
+      n += t.count(r) - t.first_with(r, x);
+    }
+    return wave_sum(n) - cuts;
+  };
+  uint32_t x = 0, above = min(cap, most) + 1;  // at_least(x) > rank >= at_least(above)
+  // Where all tiles fit the chip at once their order does not matter.
+  const bool any_order = all + pieces <= p.share;
+  while (!any_order && above - x > 1) {
+    const uint32_t mid = (x + above) / 2;
+    (at_least(mid) > rank ? x : above) = mid;
+  }
+  rank -= any_order ? 0 : at_least(above);
+  for (uint32_t c0 = 0; c0 < p.batch; c0 += 64) {
+    const Rows r = rows_of(c0 + lane);
+    const uint32_t first = t.first_with(r, x);
+    const uint32_t n = scan64(t.first_with(r, above) - first);
+    const uint64_t le = __ballot(n <= rank);
+    if (le != ~0ull) {
+      const int at = __popcll(le);
+      const uint32_t before = at == 0 ? 0 : (uint32_t)__builtin_amdgcn_readlane((int)n, at - 1);
+      const uint32_t b = c0 + at, tile = (uint32_t)__builtin_amdgcn_readlane((int)first, at) + rank - before;
+      if (b >= p.batch) return false;
+      *out = {b, tile, 0, t.key_tiles(s_rows[b], tile), 0, 1, 0};
+      return true;
+    }
+    rank -= last_lane(n);
+  }
+  return false;
 }
 
 // Nonzero if an f16 of `w` is infinite or NaN.
@@ -61,6 +210,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   __shared__ __attribute__((aligned(16))) uint16_t v_lds_a[TILE], v_lds_b[TILE];
   // s_bad[st] = ti + 1: V of the masked tile ti in stage st holds a value that is not finite.
   __shared__ uint32_t s_bad[2];
+  __shared__ Rows s_rows[kPackedMaxBatch];
+  __shared__ uint32_t s_before[kPackedMaxBatch + 1], s_last;
   auto k_stage = [&](int st) __attribute__((always_inline)) -> uint16_t * { return st ? k_lds_b : k_lds_a; };
   auto v_stage = [&](int st) __attribute__((always_inline)) -> uint16_t * { return st ? v_lds_b : v_lds_a; };
 
@@ -82,34 +233,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
       rest = id / H;
     }
   }
-  // The sequence and row tile of `rest`, by the prefix sums of the sequences' tiles.
-  uint32_t b = 0, tile = 0;
-  {
-    uint32_t before = 0;
-    bool found = false;
-    for (uint32_t c0 = 0; c0 < p.batch && !found; c0 += 64) {
-      const uint32_t bb = c0 + lane;
-      uint32_t x = bb < p.batch ? row_tiles_of(sequence_rows(p.row_starts, bb, p.rows), G) : 0;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t y = __shfl_up(x, d, 64);
-        if (lane >= d) x += y;
-      }
-      const uint64_t le = __ballot(before + x <= rest);
-      if (le != ~0ull) {
-        const int at = __popcll(le);  // x is nondecreasing
-        const uint32_t below = at == 0 ? 0 : (uint32_t)__builtin_amdgcn_readlane((int)x, at - 1);
-        b = c0 + at;
-        tile = rest - before - below;
-        found = b < p.batch;
-        break;
-      }
-      before += (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
-    }
-    if (!found) return;
+  // The sequences' rows and first positions (every wave writes all of them, and reads back
+  // what it wrote itself), and the piece of this rank.
+  for (uint32_t c0 = 0; c0 < p.batch; c0 += 64) {
+    const uint32_t bb = c0 + lane;
+    if (bb >= p.batch) continue;
+    const RowRange r = sequence_rows(p.row_starts, bb, p.rows);
+    const uint32_t tokens = r.end - r.begin;
+    s_rows[bb] = {tokens * G, PAGED ? (int32_t)paged_length(p.kv, bb) - (int32_t)tokens : 0};
   }
-  b = __builtin_amdgcn_readfirstlane(b);
-  tile = __builtin_amdgcn_readfirstlane(tile);
+  Piece pc;
+  if (!plan_piece(p, rest, s_rows, s_before, lane, &pc)) return;
+  const uint32_t b = __builtin_amdgcn_readfirstlane(pc.b), tile = __builtin_amdgcn_readfirstlane(pc.tile);
+  const uint32_t t_begin = __builtin_amdgcn_readfirstlane(pc.begin), t_end = __builtin_amdgcn_readfirstlane(pc.end);
   const RowRange range = sequence_rows(p.row_starts, b, p.rows);
   const uint32_t tokens = range.end - range.begin;
   const uint32_t L = PAGED ? paged_length(p.kv, b) : tokens;
@@ -120,7 +256,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   const bool row_ok = my_t < tokens;
   const uint32_t t_first = row0 / G, t_last = min(tokens - 1, (row0 + BM - 1) / G);
   const uint32_t kmax = p.causal != 0 ? (uint32_t)max((int64_t)0, off + t_last + 1) : L;  // at most L
-  const uint32_t n_tiles = (kmax + BN - 1) / BN;
+  const bool active = row0 + wave * 32 < tokens * G;  // whether this wave has rows
   // Last key that this lane's row sees, and that the tile's first row does.
   const int64_t lim = p.causal != 0 ? off + min(my_t, tokens - 1) : (int64_t)L - 1;
   const int64_t full_lim = p.causal != 0 ? off + t_first : (int64_t)L - 1;
@@ -160,7 +296,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     v_off[i] = ((uint32_t)r * (uint32_t)p.kv.v_pos + ((pc ^ v_swizzle<D>(row)) * 8)) * 2u;
   }
   auto issue_tile = [&](uint32_t ti, int stage) __attribute__((always_inline)) {
-    if (PAGED && (ti & 15) == 0) load_ids(ti);
+    if (PAGED && ((ti & 15) == 0 || ti == t_begin)) load_ids(ti & ~15u);
     const uint32_t key = ti * BN + wave * 16;
     const char *kt, *vt;
     bool there = key < kmax;
@@ -195,7 +331,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     }
   };
   // Tiles wholly inside the first row's window need no mask.
-  const uint32_t n_full = full_lim < 0 ? 0 : (uint32_t)min((int64_t)n_tiles, (full_lim + 1) / BN);
+  const uint32_t n_full = full_lim < 0 ? 0 : (uint32_t)min((int64_t)t_end, (full_lim + 1) / BN);
   // A masked tile's V may hold values that some of its rows must not see and that are
   // not finite, and 0 times those is NaN: each wave looks at the 16 rows it has loaded.
   auto look = [&](uint32_t ti, int stage) __attribute__((always_inline)) {
@@ -231,167 +367,169 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     const uint16_t *k_lds = ST ? k_lds_b : k_lds_a;
     const uint16_t *v_lds = ST ? v_lds_b : v_lds_a;
     const uint32_t gone = ST ? gone_b : gone_a;
-    // S^T[key][row]: two 32-key halves, at raised wave priority.
-    __builtin_amdgcn_s_setprio(1);
-    float16_t s[2];
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[mt][r] = 0.0f;
-#pragma unroll
-      for (int c = 0; c < DC; ++c) {
-        const uint16_t *kp = k_lds + (32 * mt + n) * D + (((2 * c + h) ^ k_swizzle<D>(n)) * 8);
-        s[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(*reinterpret_cast<const uint4 *>(kp)), qop[c], s[mt], 0, 0, 0);
-      }
-    }
-    __builtin_amdgcn_sched_group_barrier(kSchedDsRead, kReadAhead, 0);
-#pragma unroll
-    for (int k = 0; k < 2 * DC - kReadAhead; ++k) {
-      __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(kSchedMfma, kReadAhead, 0);
-    __builtin_amdgcn_s_setprio(0);
-    // Key 32 mt + 8 (r >> 2) + 4 h + (r & 3) of the tile is seen when it is at most
-    // lim_rel; the lane's 4 h moves to the limit, so each compare is with a constant.
-    int lim_lane = BN;
-    if constexpr (MASK) {
-      lim_lane = (int)max(min(lim - (int64_t)j0, (int64_t)BN), (int64_t)-1) - 4 * h;
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[mt][r] = 32 * mt + 8 * (r >> 2) + (r & 3) > lim_lane ? -INFINITY : s[mt][r];
-    }
-    if (PAGED && gone != 0) {
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (gone >> (2 * mt + (r >> 3)) & 1) s[mt][r] = -INFINITY;
-    }
-    // P = 2^(s c2 - m c2 + kBias) against the row's reference max m_run, as f16 pairs
-    // in accumulator order.
-    uint32_t pw[2][8];
-    float psum;
-    auto weights = [&](float mc) __attribute__((always_inline)) {
-      float ps0 = 0.0f, ps1 = 0.0f;
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-          const uint32_t w = pack_f16x2(exp2_raw(fmaf(s[mt][r], c2, -mc)), exp2_raw(fmaf(s[mt][r + 1], c2, -mc)));
-          pw[mt][r >> 1] = w;
-          if (r & 2)
-            ps1 = dot2(w, 0x3c003c00u, ps1);
-          else
-            ps0 = dot2(w, 0x3c003c00u, ps0);
-        }
-      psum = ps0 + ps1;
-    };
-    // The reference moves only when a weight leaves f16's range: the sum is then +inf
-    // or NaN, as it is for a row without a reference yet (m_run = -inf).
-    weights(m_run * c2 - kBias);
-    if (__any(!(psum <= __FLT_MAX__))) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[mt][r]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float m_new = fmaxf(m_run, mx);
-      // A row that has seen no key yet keeps m = -inf and nothing to rescale.
-      const float alpha = m_new == -INFINITY ? 1.0f : exp2_raw((m_run - m_new) * c2);
-      l_run *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
-      m_run = m_new;
-      weights(m_run == -INFINITY ? 0.0f : m_run * c2 - kBias);
-    }
-    l_run += psum;
-    // O^T[d][row] += V^T[d][keys] P^T[keys][row], four 16-key chunks.
-    auto pv = [&](auto bad_tag) __attribute__((always_inline)) {
-      constexpr bool BAD = decltype(bad_tag)::value;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int mt = c >> 1, base = (c & 1) * 4;
-        const h8_t pb = as_h8(make_uint4(pw[mt][base], pw[mt][base + 1], pw[mt][base + 2], pw[mt][base + 3]));
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const uint16_t *v0 = v_lds + 16 * c * D + tr_off + ((4 * dt + tr_chunk) ^ v_swizzle<D>(tr_key)) * 8;
-          uint2 lo = read_tr16(v0), hi = read_tr16(v0 + 8 * D);
-          if constexpr (BAD) {
-            lo = make_uint2(finite_part(lo.x), finite_part(lo.y));
-            hi = make_uint2(finite_part(hi.x), finite_part(hi.y));
-          }
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(make_uint4(lo.x, lo.y, hi.x, hi.y)), pb, o[dt], 0, 0, 0);
-        }
-      }
-    };
-    bool bad = false;
-    if constexpr (MASK) bad = s_bad[ST] == it + 1;
-    if (!bad) {
+    if (active) {
+      // S^T[key][row]: two 32-key halves, at raised wave priority.
       __builtin_amdgcn_s_setprio(1);
-      pv(std::false_type{});
-      __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2 * kReadAhead, 1);
+      float16_t s[2];
 #pragma unroll
-      for (int k = 0; k < 4 * DT - kReadAhead; ++k) {
-        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 1);
-        __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2, 1);
+      for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[mt][r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+          const uint16_t *kp = k_lds + (32 * mt + n) * D + (((2 * c + h) ^ k_swizzle<D>(n)) * 8);
+          s[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(*reinterpret_cast<const uint4 *>(kp)), qop[c], s[mt], 0, 0, 0);
+        }
       }
-      __builtin_amdgcn_sched_group_barrier(kSchedMfma, kReadAhead, 1);
+      __builtin_amdgcn_sched_group_barrier(kSchedDsRead, kReadAhead, 0);
+#pragma unroll
+      for (int k = 0; k < 2 * DC - kReadAhead; ++k) {
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(kSchedMfma, kReadAhead, 0);
       __builtin_amdgcn_s_setprio(0);
-    } else {
-      // The finite values by the products, the others added to the rows that see their
-      // key (a positive weight leaves an infinity or NaN what it is).
-      pv(std::true_type{});
-#pragma unroll 1
-      for (int key = 0; key < BN; ++key) {
-        const bool seen = key - 4 * h <= lim_lane;
+      // Key 32 mt + 8 (r >> 2) + 4 h + (r & 3) of the tile is seen when it is at most
+      // lim_rel; the lane's 4 h moves to the limit, so each compare is with a constant.
+      int lim_lane = BN;
+      if constexpr (MASK) {
+        lim_lane = (int)max(min(lim - (int64_t)j0, (int64_t)BN), (int64_t)-1) - 4 * h;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[mt][r] = 32 * mt + 8 * (r >> 2) + (r & 3) > lim_lane ? -INFINITY : s[mt][r];
+      }
+      if (PAGED && gone != 0) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (gone >> (2 * mt + (r >> 3)) & 1) s[mt][r] = -INFINITY;
+      }
+      // P = 2^(s c2 - m c2 + kBias) against the row's reference max m_run, as f16 pairs
+      // in accumulator order.
+      uint32_t pw[2][8];
+      float psum;
+      auto weights = [&](float mc) __attribute__((always_inline)) {
+        float ps0 = 0.0f, ps1 = 0.0f;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int r = 0; r < 16; r += 2) {
+            const uint32_t w = pack_f16x2(exp2_raw(fmaf(s[mt][r], c2, -mc)), exp2_raw(fmaf(s[mt][r + 1], c2, -mc)));
+            pw[mt][r >> 1] = w;
+            if (r & 2)
+              ps1 = dot2(w, 0x3c003c00u, ps1);
+            else
+              ps0 = dot2(w, 0x3c003c00u, ps0);
+          }
+        psum = ps0 + ps1;
+      };
+      // The reference moves only when a weight leaves f16's range: the sum is then +inf
+      // or NaN, as it is for a row without a reference yet (m_run = -inf).
+      weights(m_run * c2 - kBias);
+      if (__any(!(psum <= __FLT_MAX__))) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[mt][r]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float m_new = fmaxf(m_run, mx);
+        // A row that has seen no key yet keeps m = -inf and nothing to rescale.
+        const float alpha = m_new == -INFINITY ? 1.0f : exp2_raw((m_run - m_new) * c2);
+        l_run *= alpha;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            // d = 32 dt + 8 q + 4 h + e of this lane's row.
-            const int chunk = (4 * dt + q) ^ v_swizzle<D>(key);
-            const uint2 v = *reinterpret_cast<const uint2 *>(v_lds + key * D + chunk * 8 + 4 * h);
-            const uint32_t w[2] = {v.x, v.y};
+          for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+        m_run = m_new;
+        weights(m_run == -INFINITY ? 0.0f : m_run * c2 - kBias);
+      }
+      l_run += psum;
+      // O^T[d][row] += V^T[d][keys] P^T[keys][row], four 16-key chunks.
+      auto pv = [&](auto bad_tag) __attribute__((always_inline)) {
+        constexpr bool BAD = decltype(bad_tag)::value;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint16_t x = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-              if (seen && (x & 0x7c00u) == 0x7c00u) o[dt][4 * q + e] += f16_to_f32(x);
+        for (int c = 0; c < 4; ++c) {
+          const int mt = c >> 1, base = (c & 1) * 4;
+          const h8_t pb = as_h8(make_uint4(pw[mt][base], pw[mt][base + 1], pw[mt][base + 2], pw[mt][base + 3]));
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            const uint16_t *v0 = v_lds + 16 * c * D + tr_off + ((4 * dt + tr_chunk) ^ v_swizzle<D>(tr_key)) * 8;
+            uint2 lo = read_tr16(v0), hi = read_tr16(v0 + 8 * D);
+            if constexpr (BAD) {
+              lo = make_uint2(finite_part(lo.x), finite_part(lo.y));
+              hi = make_uint2(finite_part(hi.x), finite_part(hi.y));
             }
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(make_uint4(lo.x, lo.y, hi.x, hi.y)), pb, o[dt], 0, 0, 0);
           }
+        }
+      };
+      bool bad = false;
+      if constexpr (MASK) bad = s_bad[ST] == it + 1;
+      if (!bad) {
+        __builtin_amdgcn_s_setprio(1);
+        pv(std::false_type{});
+        __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2 * kReadAhead, 1);
+#pragma unroll
+        for (int k = 0; k < 4 * DT - kReadAhead; ++k) {
+          __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 1);
+          __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2, 1);
+        }
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, kReadAhead, 1);
+        __builtin_amdgcn_s_setprio(0);
+      } else {
+        // The finite values by the products, the others added to the rows that see their
+        // key (a positive weight leaves an infinity or NaN what it is).
+        pv(std::true_type{});
+#pragma unroll 1
+        for (int key = 0; key < BN; ++key) {
+          const bool seen = key - 4 * h <= lim_lane;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              // d = 32 dt + 8 q + 4 h + e of this lane's row.
+              const int chunk = (4 * dt + q) ^ v_swizzle<D>(key);
+              const uint2 v = *reinterpret_cast<const uint2 *>(v_lds + key * D + chunk * 8 + 4 * h);
+              const uint32_t w[2] = {v.x, v.y};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint16_t x = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+                if (seen && (x & 0x7c00u) == 0x7c00u) o[dt][4 * q + e] += f16_to_f32(x);
+              }
+            }
+        }
       }
     }
     // Tile it + 1 (issued a tile ago) has landed in this wave's part of the other stage;
     // after the barrier nobody reads this stage, which then receives tile it + 2.
     wait_vmcnt<0>();
-    if (it + 1 < n_tiles) look(it + 1, ST ^ 1);
+    if (it + 1 < t_end) look(it + 1, ST ^ 1);
     __syncthreads();
-    if (it + 2 < n_tiles) issue_tile(it + 2, ST);
+    if (it + 2 < t_end) issue_tile(it + 2, ST);
   };
 
-  if (n_tiles > 0) {
+  if (t_begin < t_end) {
     if (tid < 2) s_bad[tid] = 0;
     __syncthreads();
-    // The first tile is computed once it has landed; the second stays in flight. Loads
-    // complete in issue order, so vmcnt(2 BPW) leaves only the second tile's pending. The
-    // barrier is a bare s_barrier (a workgroup fence would wait for every load); each
+    // The first tile (stage 0) is computed once it has landed; the second stays in flight.
+    // Loads complete in issue order, so vmcnt(2 BPW) leaves only the second tile's pending.
+    // The barrier is a bare s_barrier (a workgroup fence would wait for every load); each
     // wave has waited for its own part, and the memory clobber keeps LDS reads below it.
-    issue_tile(0, 0);
-    if (n_tiles > 1) {
-      issue_tile(1, 1);
+    issue_tile(t_begin, 0);
+    if (t_begin + 1 < t_end) {
+      issue_tile(t_begin + 1, 1);
       wait_vmcnt<2 * BPW>();
     } else {
       wait_vmcnt<0>();
     }
-    look(0, 0);
+    look(t_begin, 0);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     using S0 = std::integral_constant<int, 0>;
     using S1 = std::integral_constant<int, 1>;
-    uint32_t it = 0;
+    uint32_t it = t_begin;
     for (; it + 1 < n_full; it += 2) {
       step(it, std::false_type{}, S0{});
       step(it + 1, std::false_type{}, S1{});
@@ -400,18 +538,79 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
       step(it, std::false_type{}, S0{});
       ++it;
     }
-    if ((it & 1) != 0 && it < n_tiles) {
+    if (((it - t_begin) & 1) != 0 && it < t_end) {
       step(it, std::true_type{}, S1{});
       ++it;
     }
-    for (; it + 1 < n_tiles; it += 2) {
+    for (; it + 1 < t_end; it += 2) {
       step(it, std::true_type{}, S0{});
       step(it + 1, std::true_type{}, S1{});
     }
-    if (it < n_tiles) step(it, std::true_type{}, S0{});
+    if (it < t_end) step(it, std::true_type{}, S0{});
   }
 
-  const float l_total = l_run + __shfl_xor(l_run, 32, 64);
+  float l_total = l_run + __shfl_xor(l_run, 32, 64);
+  const uint32_t pieces = __builtin_amdgcn_readfirstlane(pc.pieces), piece = __builtin_amdgcn_readfirstlane(pc.piece);
+  if (pieces > 1) {
+    // This piece's rows, in the accumulators' own order so that a store's lanes are
+    // neighbours: per wave 8-byte slots of 64 lanes, (m, l) and then O two by two. A row
+    // that saw no key here has m = -inf.
+    constexpr uint32_t WAVE = packed_partial_slots(D) * 64 * 2, PIECE = 4 * WAVE;
+    float *first = p.partial + ((size_t)kvh * p.max_pieces + (rest - piece)) * PIECE + wave * WAVE + lane * 2;
+    if (active) {
+      float *mine = first + (size_t)piece * PIECE;
+      store_partial2(mine, m_run, l_total);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) store_partial2(mine + (1 + 8 * dt + r / 2) * 128, o[dt][r], o[dt][r + 1]);
+    }
+    wait_vmcnt<0>();
+    __syncthreads();
+    if (tid == 0) {
+      uint32_t *counter = p.counters + (size_t)(kvh * p.max_pieces + pc.cut) * p.counter_stride;
+      const bool last = arrive(counter) == pieces - 1;
+      if (last) {
+        acquire_partials();
+        __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      s_last = last;
+    }
+    __syncthreads();
+    if (s_last == 0) return;
+    // The last piece of the tile to finish joins all of them, in order.
+    if (active) {
+      float2 ml[kMostPieces];
+#pragma unroll
+      for (uint32_t k = 0; k < kMostPieces; ++k) ml[k] = load_partial2(first + (size_t)min(k, pieces - 1) * PIECE);
+      float M = -INFINITY;
+#pragma unroll
+      for (uint32_t k = 0; k < kMostPieces; ++k) M = fmaxf(M, ml[k].x);
+      l_total = 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
+#pragma unroll 1
+      for (uint32_t k = 0; k < pieces; ++k) {
+        const float *from = first + (size_t)k * PIECE;
+        const float2 own = load_partial2(from);
+        float2 v[8 * DT];
+#pragma unroll
+        for (int i = 0; i < 8 * DT; ++i) v[i] = load_partial2(from + (1 + i) * 128);
+        if (own.x == -INFINITY) continue;
+        const float f = exp2_raw((own.x - M) * c2);
+        l_total = fmaf(own.y, f, l_total);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; r += 2) {
+            o[dt][r] = fmaf(v[8 * dt + r / 2].x, f, o[dt][r]);
+            o[dt][r + 1] = fmaf(v[8 * dt + r / 2].y, f, o[dt][r + 1]);
+          }
+      }
+    }
+  }
   // Normalise (a row that saw no key: 0 / 0), then store through LDS: each wave writes
   // its 32 rows as f16 into a region of the idle stages and stores them back as whole
   // 16-byte chunks, D / 8 consecutive lanes per row.
@@ -446,12 +645,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
 
 template <int D>
 hipError_t launch_d(const PackedParams &p, const Launch &l) {
-  const dim3 grid(p.row_tiles * p.kv_heads);
+  const dim3 grid((p.row_tiles + p.max_pieces) * p.kv_heads);
   return p.kv.table != nullptr ? dispatch(attn_packed_kernel<D, true>, grid, dim3(256), 0, l, p)
                                : dispatch(attn_packed_kernel<D, false>, grid, dim3(256), 0, l, p);
 }
 
 }  // namespace
+
+uint32_t packed_workgroups(uint32_t compute_units, uint32_t head_dim) {
+  return (head_dim == 256 ? 1 : 2) * (compute_units > 1 ? compute_units : 1);
+}
 
 uint64_t packed_row_tiles(uint64_t rows, uint32_t batch, uint32_t group) {
   return rows * group / BM + (batch < rows ? batch : rows);

@@ -42,17 +42,6 @@ constexpr uint32_t kPiece = kWaves, kShare = 2;
 // steps of kJoin.
 constexpr uint32_t kManyUnits = 128, kJoin = 16;
 
-// Sum of x over the lanes up to this one (row shifts, then the rows' last lanes).
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_add(uint32_t x) {
-  return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ uint32_t scan64(uint32_t x) {
-  x = dpp_add<0x118, 0xf>(dpp_add<0x114, 0xf>(dpp_add<0x112, 0xf>(dpp_add<0x111, 0xf>(x))));
-  return dpp_add<0x143, 0xc>(dpp_add<0x142, 0xa>(x));
-}
-__device__ __forceinline__ uint32_t last_lane(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); }
-
 __device__ __forceinline__ float lane_value(float x, int lane) {
   return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), lane));
 }

@@ -216,13 +216,36 @@ mi_status packed(mi_batch *batch, const mi_tensor *q, const mi_tensor *key, cons
   p.q_heads = config->query_heads, p.kv_heads = config->kv_heads, p.group = p.q_heads / p.kv_heads;
   p.causal = config->causal != 0 ? 1 : 0;
   p.scale_log2 = scale_log2(config->head_dim);
-  const uint64_t tiles = kernels::packed_row_tiles(p.rows, p.batch, p.group);
-  if ((uint64_t)p.rows * p.group >= kRows31 || tiles * p.kv_heads >= kRows31)
+  // Sequences beyond one launch's go in launches of their own, each with room for all rows.
+  const uint32_t step = std::min(p.batch, kernels::kPackedMaxBatch);
+  const uint64_t tiles = kernels::packed_row_tiles(p.rows, step, p.group);
+  if ((uint64_t)p.rows * p.group >= kRows31 || tiles * p.kv_heads + kernels::kSplitCounters >= kRows31)
     return fail(MI_ERR_SHAPE, "attention grid exceeds the launch limits");
   if ((st = check_batch(batch)) != MI_OK || q->shape[0] == 0 || sequences == 0) return st;
   p.row_tiles = (uint32_t)tiles;
-  return launch(batch, paged ? "attn_paged" : "attn_packed",
-                [&](const kernels::Launch &s) { return kernels::launch_packed(p, config->head_dim, s); });
+  // Twice the workgroups that run at once: an even share each, and a last piece per tile.
+  Context *ctx = batch->ctx;
+  p.share = std::max(1u, kernels::packed_workgroups(ctx->compute_units, config->head_dim) / p.kv_heads);
+  p.max_pieces = (uint64_t)2 * p.share * p.kv_heads <= ctx->split_counter_count ? 2 * p.share : 0;
+  p.counters = ctx->split_counters;
+  p.counter_stride = kernels::counter_stride((uint64_t)p.max_pieces * p.kv_heads, ctx->split_counter_count);
+  void *scratch = nullptr;
+  if (p.max_pieces != 0) {
+    const uint64_t floats = kernels::packed_partial_floats(p.max_pieces, p.kv_heads, config->head_dim);
+    if ((st = scratch_alloc(batch, floats * sizeof(float), &scratch)) != MI_OK) return st;
+  }
+  p.partial = static_cast<float *>(scratch);
+  for (uint32_t first = 0; first < (uint32_t)sequences && st == MI_OK; first += step) {
+    kernels::PackedParams part = p;
+    part.batch = std::min(step, p.batch - first);
+    part.row_starts += first;
+    if (paged) part.kv.table += first * p.kv.table_seq, part.kv.lengths += first;
+    st = launch(batch, paged ? "attn_paged" : "attn_packed",
+                [&](const kernels::Launch &s) { return kernels::launch_packed(part, config->head_dim, s); });
+  }
+  // In-order execution makes the range reusable by later work of the batch.
+  if (scratch != nullptr) scratch_free(ctx, scratch);
+  return st;
 }
 
 mi_status append_paged(mi_batch *batch, const mi_tensor *q, const mi_tensor *k, const mi_tensor *value,

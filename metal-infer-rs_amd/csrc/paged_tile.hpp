@@ -43,6 +43,17 @@ __device__ __forceinline__ uint32_t paged_length(const kernels::PagedKv &kv, uin
   return min(kv.lengths[b], kv.table_width << kv.page_shift);
 }
 
+// Sum of x over the lanes up to this one (row shifts, then the rows' last lanes).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t x) {
+  return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t scan64(uint32_t x) {
+  x = dpp_add<0x118, 0xf>(dpp_add<0x114, 0xf>(dpp_add<0x112, 0xf>(dpp_add<0x111, 0xf>(x))));
+  return dpp_add<0x143, 0xc>(dpp_add<0x142, 0xa>(x));
+}
+__device__ __forceinline__ uint32_t last_lane(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); }
+
 // The parameters of a kernel of one parameter, read again: what is used only before and
 // after a loop then takes none of its scalar registers (the compiler would keep every
 // parameter from the first read to the last use, and spill).
