@@ -32,7 +32,9 @@ namespace {
 
 using namespace mi::dev;
 
-constexpr int BN = kPrefillBlockN;  // keys per tile
+// Keys per tile: at head_dim 256 half as many, as the accumulators and Q take half of a
+// wave's registers.
+constexpr int tile_keys(int head_dim) { return head_dim == 256 ? 32 : kPrefillBlockN; }
 constexpr int BM = kPrefillBlockM;  // rows per workgroup
 // Added to every weight's exponent, so that f16 holds weights down to 2^-32 of the
 // reference's (a long tail of them counts); it cancels against the row sum.
@@ -42,40 +44,50 @@ constexpr uint32_t kLeastPiece = 4, kMostPieces = 16;
 constexpr int kReadAhead = 4;       // LDS operand reads in flight ahead of the MFMAs
 constexpr int kSchedMfma = 0x008, kSchedDsRead = 0x100;
 
-// A sequence as the plan sees it: its packed (token, head) rows, and the position of its
-// first row (negative: more rows than keys).
+// A sequence as the plan sees it: its row tiles, the key tiles of the first and of the
+// last of them, and the position of its first row (negative: more rows than keys).
 struct Rows {
-  uint32_t rows;
+  uint32_t tiles, least, most;
   int32_t first;
 };
 
-// Row tiles and their 64-key tiles.
+// Key tiles of the row tiles of one sequence. Under the causal mask they grow from tile
+// to tile, else all are the same.
+template <int BN>
 struct Tiles {
   uint32_t group, causal;
-  __device__ __forceinline__ uint32_t count(Rows r) const { return (r.rows + BM - 1) / BM; }
-  // Keys that the last row of tile i sees.
-  __device__ __forceinline__ uint32_t keys(Rows r, uint32_t i) const {
-    const int32_t tokens = (int32_t)(r.rows / group);
-    const int32_t last = causal != 0 ? min(tokens - 1, (int32_t)(((i + 1) * BM - 1) / group)) : tokens - 1;
-    return (uint32_t)max(0, r.first + last + 1);
+  // Keys that the last row of tile i sees, of `tokens` tokens.
+  __device__ __forceinline__ uint32_t of(int32_t first, uint32_t tokens, uint32_t i) const {
+    const uint32_t last = causal != 0 ? min(tokens - 1, ((i + 1) * BM - 1) / group) : tokens - 1;
+    return ((uint32_t)max(0, first + (int32_t)last + 1) + BN - 1) / BN;
   }
-  __device__ __forceinline__ uint32_t key_tiles(Rows r, uint32_t i) const { return (keys(r, i) + BN - 1) / BN; }
-  // The first row tile with at least x key tiles (the count of them if none has).
+  __device__ __forceinline__ Rows sequence(int32_t first, uint32_t tokens) const {
+    const uint32_t n = (tokens * group + BM - 1) / BM;
+    return n == 0 ? Rows{0, 0, 0, 0} : Rows{n, of(first, tokens, 0), of(first, tokens, n - 1), first};
+  }
+  // The first row tile with at least x key tiles (the count of them if none has): that of
+  // the first token that sees key (x - 1) BN.
   __device__ __forceinline__ uint32_t first_with(Rows r, uint32_t x) const {
-    const uint32_t all = count(r);
-    if (all == 0 || key_tiles(r, 0) >= x) return 0;
-    if (key_tiles(r, all - 1) < x) return all;
-    // Causal, x > 0: the tile of the first token that sees key (x - 1) BN.
-    return (uint32_t)((int32_t)((x - 1) * BN) - r.first) * group / BM;
+    const uint32_t i = (uint32_t)((int32_t)((x - 1) * BN) - r.first) * group / BM;
+    return x <= r.least ? 0 : x > r.most ? r.tiles : i;
+  }
+  // Key tiles of tile i.
+  __device__ __forceinline__ uint32_t at(Rows r, uint32_t i) const {
+    if (causal == 0 || i + 1 >= r.tiles) return r.most;
+    const int32_t last = (int32_t)(((i + 1) * BM - 1) / group);
+    return ((uint32_t)max(0, r.first + last + 1) + BN - 1) / BN;
   }
 };
 
-// Sums and the like over the 64 lanes, to every lane.
+// Sum and largest value over the 64 lanes, to every lane.
 __device__ __forceinline__ uint32_t wave_sum(uint32_t x) { return last_lane(scan64(x)); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false));
+}
 __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x = max(x, (uint32_t)__shfl_xor((int)x, d, 64));
-  return x;
+  x = dpp_max<0x118, 0xf>(dpp_max<0x114, 0xf>(dpp_max<0x112, 0xf>(dpp_max<0x111, 0xf>(x))));
+  return last_lane(dpp_max<0x143, 0xc>(dpp_max<0x142, 0xa>(x)));
 }
 
 // What the workgroup of a rank does: key tiles [begin, end) of a row tile, as piece
@@ -86,19 +98,27 @@ struct Piece {
 
 // The piece of `rank` (of one KV head), the same in every wave that asks. `share`: the
 // workgroups that the chip runs at once for one KV head.
-__device__ __forceinline__ bool plan_piece(const PackedParams &p, uint32_t rank, const Rows *s_rows, uint32_t *s_before, int lane,
-                           Piece *out) {
-  const Tiles t{p.group, p.causal};
-  auto rows_of = [&](uint32_t b) { return b < p.batch ? s_rows[b] : Rows{0, 0}; };
+template <int BN>
+__device__ __forceinline__ bool plan_piece(const PackedParams &p, uint32_t rank, const Rows *s_rows,
+                                           uint32_t *s_before, int lane, Piece *out) {
+  const Tiles<BN> t{p.group, p.causal};
+  // The first 64 sequences stay in registers.
+  const uint32_t own = min((uint32_t)lane, p.batch - 1);
+  const bool is_own = (uint32_t)lane < p.batch;
+  const uint32_t tiles = is_own ? s_rows[own].tiles : 0, least = s_rows[own].least, longest = is_own ? s_rows[own].most : 0;
+  const int32_t start = s_rows[own].first;
+  auto rows_of = [&](uint32_t c0) __attribute__((always_inline)) -> Rows {
+    if (c0 == 0) return Rows{tiles, least, longest, start};
+    const bool is = c0 + lane < p.batch;
+    const uint32_t at = is ? c0 + lane : 0;
+    return Rows{is ? s_rows[at].tiles : 0, s_rows[at].least, is ? s_rows[at].most : 0, s_rows[at].first};
+  };
   uint32_t all = 0, most = 0, work = 0;  // row tiles; key tiles of the longest; of all (about)
   for (uint32_t c0 = 0; c0 < p.batch; c0 += 64) {
-    const Rows r = rows_of(c0 + lane);
-    const uint32_t n = t.count(r);
-    if (n == 0) continue;
-    const uint32_t lo = t.key_tiles(r, 0), hi = t.key_tiles(r, n - 1);
-    all += n;
-    most = max(most, hi);
-    work += n * (lo + hi + 1) / 2;
+    const Rows r = rows_of(c0);
+    all += r.tiles;
+    most = max(most, r.most);
+    work += r.tiles * (r.least + r.most + 1) / 2;
   }
   all = wave_sum(all), most = wave_max(most), work = wave_sum(work);
   if (rank >= all + p.max_pieces) return false;
@@ -118,8 +138,8 @@ __device__ __forceinline__ bool plan_piece(const PackedParams &p, uint32_t rank,
     found = false;
     if (cap >= most) break;
     for (uint32_t c0 = 0; c0 < p.batch; c0 += 64) {
-      const Rows r = rows_of(c0 + lane);
-      const uint32_t x = scan64(t.count(r) - t.first_with(r, cap + 1));
+      const Rows r = rows_of(c0);
+      const uint32_t x = scan64(r.tiles - t.first_with(r, cap + 1));
       if (c0 + lane < p.batch) s_before[c0 + lane + 1] = cuts + x;
       cuts += last_lane(x);
     }
@@ -130,9 +150,9 @@ __device__ __forceinline__ bool plan_piece(const PackedParams &p, uint32_t rank,
       uint32_t lo = 0;  // the last sequence with s_before[lo] <= k
       for (uint32_t step = 512; step != 0; step >>= 1)
         if (lo + step < p.batch && s_before[lo + step] <= k) lo += step;
-      const Rows r = rows_of(lo);
+      const Rows r = s_rows[lo];
       const uint32_t i = k < cuts ? t.first_with(r, cap + 1) + k - s_before[lo] : 0;
-      const uint32_t n = k < cuts ? t.key_tiles(r, i) : 0, s = (n + cap - 1) / cap;
+      const uint32_t n = k < cuts ? t.at(r, i) : 0, s = (n + cap - 1) / cap;
       const uint32_t x = scan64(s);
       const uint64_t le = __ballot(pieces + x <= rank);
       if (!found && le != ~0ull) {
@@ -156,8 +176,8 @@ __device__ __forceinline__ bool plan_piece(const PackedParams &p, uint32_t rank,
   auto at_least = [&](uint32_t x) -> uint32_t {
     uint32_t n = 0;
     for (uint32_t c0 = 0; c0 < p.batch; c0 += 64) {
-      const Rows r = rows_of(c0 + lane);
-      n += t.count(r) - t.first_with(r, x);
+      const Rows r = rows_of(c0);
+      n += r.tiles - t.first_with(r, x);
     }
     return wave_sum(n) - cuts;
   };
@@ -170,7 +190,7 @@ __device__ __forceinline__ bool plan_piece(const PackedParams &p, uint32_t rank,
   }
   rank -= any_order ? 0 : at_least(above);
   for (uint32_t c0 = 0; c0 < p.batch; c0 += 64) {
-    const Rows r = rows_of(c0 + lane);
+    const Rows r = rows_of(c0);
     const uint32_t first = t.first_with(r, x);
     const uint32_t n = scan64(t.first_with(r, above) - first);
     const uint64_t le = __ballot(n <= rank);
@@ -179,7 +199,7 @@ __device__ __forceinline__ bool plan_piece(const PackedParams &p, uint32_t rank,
       const uint32_t before = at == 0 ? 0 : (uint32_t)__builtin_amdgcn_readlane((int)n, at - 1);
       const uint32_t b = c0 + at, tile = (uint32_t)__builtin_amdgcn_readlane((int)first, at) + rank - before;
       if (b >= p.batch) return false;
-      *out = {b, tile, 0, t.key_tiles(s_rows[b], tile), 0, 1, 0};
+      *out = {b, tile, 0, t.at(s_rows[b], tile), 0, 1, 0};
       return true;
     }
     rank -= last_lane(n);
@@ -200,13 +220,16 @@ __device__ __forceinline__ uint32_t finite_part(uint32_t w) {
 template <int D, bool PAGED>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(const PackedParams p) {
   constexpr int CPR = D / 8;           // 16-byte chunks per tile row
+  constexpr int BN = tile_keys(D), MT = BN / 32;
   constexpr int RPB = 512 / D;         // tile rows per 1 KB direct load
-  constexpr int BPW = 16 / RPB;        // direct loads of K (and V) per wave and tile
+  constexpr int RPW = BN / 4;          // tile rows that a wave loads
+  constexpr int BPW = RPW / RPB;       // its direct loads of K (and V) per tile
+  constexpr uint32_t GROUPS = BN / 16, HELD = 64 / GROUPS;  // 16-key groups per tile; tiles whose page ids a wave holds
   constexpr int DC = D / 16, DT = D / 32;
-  constexpr int TILE = BN * D;
+  constexpr int TILE = BN * D, OUT = 64 * D;  // halves of a tile, and of two waves' output rows
   // One array per stage, and the stage a compile-time choice, so that the compiler can
   // tell the loads into one from the reads of the other.
-  __shared__ __attribute__((aligned(16))) uint16_t k_lds_a[TILE], k_lds_b[TILE];
+  __shared__ __attribute__((aligned(16))) uint16_t k_lds_a[OUT], k_lds_b[OUT];
   __shared__ __attribute__((aligned(16))) uint16_t v_lds_a[TILE], v_lds_b[TILE];
   // s_bad[st] = ti + 1: V of the masked tile ti in stage st holds a value that is not finite.
   __shared__ uint32_t s_bad[2];
@@ -240,10 +263,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     if (bb >= p.batch) continue;
     const RowRange r = sequence_rows(p.row_starts, bb, p.rows);
     const uint32_t tokens = r.end - r.begin;
-    s_rows[bb] = {tokens * G, PAGED ? (int32_t)paged_length(p.kv, bb) - (int32_t)tokens : 0};
+    s_rows[bb] = Tiles<BN>{G, p.causal}.sequence(PAGED ? (int32_t)paged_length(p.kv, bb) - (int32_t)tokens : 0, tokens);
   }
   Piece pc;
-  if (!plan_piece(p, rest, s_rows, s_before, lane, &pc)) return;
+  if (!plan_piece<BN>(p, rest, s_rows, s_before, lane, &pc)) return;
   const uint32_t b = __builtin_amdgcn_readfirstlane(pc.b), tile = __builtin_amdgcn_readfirstlane(pc.tile);
   const uint32_t t_begin = __builtin_amdgcn_readfirstlane(pc.begin), t_end = __builtin_amdgcn_readfirstlane(pc.end);
   const RowRange range = sequence_rows(p.row_starts, b, p.rows);
@@ -271,8 +294,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
       qop[c] = row_ok ? as_h8(*reinterpret_cast<const uint4 *>(qrow + 16 * c)) : as_h8(make_uint4(0, 0, 0, 0));
   }
 
-  // Page ids of the tiles' 16-key groups: lane l holds group l of the 64 (16 tiles)
-  // since tile 16 k. `absent` has a bit for each group without a page, gone_a / gone_b
+  // Page ids of the tiles' 16-key groups: lane l holds group l of the 64 (HELD tiles)
+  // since tile HELD k. `absent` has a bit for each group without a page, gone_a / gone_b
   // those of the tiles in the stages.
   uint32_t ids = 0, gone_a = 0, gone_b = 0;
   uint64_t absent = 0;
@@ -291,19 +314,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   uint32_t k_off[BPW], v_off[BPW];
 #pragma unroll
   for (int i = 0; i < BPW; ++i) {
-    const int r = i * RPB + lane / CPR, row = wave * 16 + r, pc = lane % CPR;
+    const int r = i * RPB + lane / CPR, row = wave * RPW + r, pc = lane % CPR;
     k_off[i] = ((uint32_t)r * (uint32_t)p.kv.k_pos + ((pc ^ k_swizzle<D>(row)) * 8)) * 2u;
     v_off[i] = ((uint32_t)r * (uint32_t)p.kv.v_pos + ((pc ^ v_swizzle<D>(row)) * 8)) * 2u;
   }
   auto issue_tile = [&](uint32_t ti, int stage) __attribute__((always_inline)) {
-    if (PAGED && ((ti & 15) == 0 || ti == t_begin)) load_ids(ti & ~15u);
-    const uint32_t key = ti * BN + wave * 16;
+    if (PAGED && (ti % HELD == 0 || ti == t_begin)) load_ids(ti / HELD * HELD);
+    const uint32_t key = ti * BN + wave * RPW;
     const char *kt, *vt;
     bool there = key < kmax;
     if constexpr (PAGED) {
-      const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)(4 * (ti & 15) + wave));
+      const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)(GROUPS * (ti % HELD) + wave * RPW / 16));
       there = there && page < p.kv.pages;
-      (stage ? gone_b : gone_a) = (uint32_t)(absent >> (4 * (ti & 15))) & 15u;
+      (stage ? gone_b : gone_a) = (uint32_t)(absent >> (GROUPS * (ti % HELD))) & ((1u << GROUPS) - 1);
       kt = reinterpret_cast<const char *>(p.kv.k + (int64_t)page * p.kv.k_page + (int64_t)(key & in_page) * p.kv.k_pos +
                                           (int64_t)kvh * p.kv.k_head);
       vt = reinterpret_cast<const char *>(p.kv.v + (int64_t)page * p.kv.v_page + (int64_t)(key & in_page) * p.kv.v_pos +
@@ -312,8 +335,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
       kt = reinterpret_cast<const char *>(p.kv.k + (int64_t)(range.begin + key) * p.kv.k_pos + (int64_t)kvh * p.kv.k_head);
       vt = reinterpret_cast<const char *>(p.kv.v + (int64_t)(range.begin + key) * p.kv.v_pos + (int64_t)kvh * p.kv.v_head);
     }
-    uint16_t *kd = k_stage(stage) + wave * 16 * D, *vd = v_stage(stage) + wave * 16 * D;
-    if (there && key + 16 <= kmax) {
+    uint16_t *kd = k_stage(stage) + wave * RPW * D, *vd = v_stage(stage) + wave * RPW * D;
+    if (there && key + RPW <= kmax) {
 #pragma unroll
       for (int i = 0; i < BPW; ++i) {
         load_lds16(reinterpret_cast<const uint16_t *>(kt + k_off[i]), kd + i * 512);
@@ -333,17 +356,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   // Tiles wholly inside the first row's window need no mask.
   const uint32_t n_full = full_lim < 0 ? 0 : (uint32_t)min((int64_t)t_end, (full_lim + 1) / BN);
   // A masked tile's V may hold values that some of its rows must not see and that are
-  // not finite, and 0 times those is NaN: each wave looks at the 16 rows it has loaded.
+  // not finite, and 0 times those is NaN. Each wave looks at the rows it has loaded: such
+  // values become zeros, and the rows that see them get them from memory (add_bad).
   auto look = [&](uint32_t ti, int stage) __attribute__((always_inline)) {
     if (ti < n_full) return;
-    const uint16_t *mine = v_stage(stage) + wave * 16 * D;
-    uint32_t bad = 0;
+    uint16_t *mine = v_stage(stage) + wave * RPW * D;
+    bool bad = false;
 #pragma unroll
     for (int i = 0; i < BPW; ++i) {
-      const uint4 v = *reinterpret_cast<const uint4 *>(mine + i * 512 + lane * 8);
-      bad |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w);
+      uint4 *at = reinterpret_cast<uint4 *>(mine + i * 512 + lane * 8);
+      const uint4 v = *at;
+      if ((not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w)) != 0) {
+        *at = make_uint4(finite_part(v.x), finite_part(v.y), finite_part(v.z), finite_part(v.w));
+        bad = true;
+      }
     }
-    if (__any(bad != 0)) s_bad[stage] = ti + 1;
+    if (__any(bad)) s_bad[stage] = ti + 1;
   };
 
   float16_t o[DT];
@@ -360,6 +388,36 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   const int tr_off = tr_key * D + 4 * (tr_a & 1);
   const int tr_chunk = 2 * (tr_g & 1) + (tr_a >> 1);
 
+  // Adds the values of the tile at key j0 that are not finite to the rows that see them (a
+  // positive weight leaves an infinity or NaN what it is).
+  auto add_bad = [&](uint32_t j0) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (uint32_t key = j0; key < min(j0 + BN, kmax); ++key) {
+      const uint16_t *row = p.kv.v + (int64_t)kvh * p.kv.v_head;
+      if constexpr (PAGED) {
+        const uint32_t page = p.kv.table[(int64_t)b * p.kv.table_seq + (key >> shift)];
+        if (page >= p.kv.pages) continue;
+        row += (int64_t)page * p.kv.v_page + (int64_t)(key & in_page) * p.kv.v_pos;
+      } else {
+        row += (int64_t)(range.begin + key) * p.kv.v_pos;
+      }
+      if ((int64_t)key > lim) continue;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          // d = 32 dt + 8 q + 4 h + e of this lane's row.
+          const uint2 v = *reinterpret_cast<const uint2 *>(row + 32 * dt + 8 * q + 4 * h);
+          const uint32_t w[2] = {v.x, v.y};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint16_t x = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+            if ((x & 0x7c00u) == 0x7c00u) o[dt][4 * q + e] += f16_to_f32(x);
+          }
+        }
+    }
+  };
+
   auto step = [&](uint32_t it, auto mask_tag, auto stage_tag) __attribute__((always_inline)) {
     constexpr bool MASK = decltype(mask_tag)::value;
     constexpr int ST = decltype(stage_tag)::value;
@@ -370,9 +428,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     if (active) {
       // S^T[key][row]: two 32-key halves, at raised wave priority.
       __builtin_amdgcn_s_setprio(1);
-      float16_t s[2];
+      float16_t s[MT];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
+      for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[mt][r] = 0.0f;
 #pragma unroll
@@ -383,7 +441,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
       }
       __builtin_amdgcn_sched_group_barrier(kSchedDsRead, kReadAhead, 0);
 #pragma unroll
-      for (int k = 0; k < 2 * DC - kReadAhead; ++k) {
+      for (int k = 0; k < MT * DC - kReadAhead; ++k) {
         __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
         __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
       }
@@ -395,25 +453,25 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
       if constexpr (MASK) {
         lim_lane = (int)max(min(lim - (int64_t)j0, (int64_t)BN), (int64_t)-1) - 4 * h;
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[mt][r] = 32 * mt + 8 * (r >> 2) + (r & 3) > lim_lane ? -INFINITY : s[mt][r];
       }
       if (PAGED && gone != 0) {
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (gone >> (2 * mt + (r >> 3)) & 1) s[mt][r] = -INFINITY;
       }
       // P = 2^(s c2 - m c2 + kBias) against the row's reference max m_run, as f16 pairs
       // in accumulator order.
-      uint32_t pw[2][8];
+      uint32_t pw[MT][8];
       float psum;
       auto weights = [&](float mc) __attribute__((always_inline)) {
         float ps0 = 0.0f, ps1 = 0.0f;
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int r = 0; r < 16; r += 2) {
             const uint32_t w = pack_f16x2(exp2_raw(fmaf(s[mt][r], c2, -mc)), exp2_raw(fmaf(s[mt][r + 1], c2, -mc)));
@@ -431,7 +489,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
       if (__any(!(psum <= __FLT_MAX__))) {
         float mx = -INFINITY;
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[mt][r]);
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
@@ -447,60 +505,29 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
         weights(m_run == -INFINITY ? 0.0f : m_run * c2 - kBias);
       }
       l_run += psum;
-      // O^T[d][row] += V^T[d][keys] P^T[keys][row], four 16-key chunks.
-      auto pv = [&](auto bad_tag) __attribute__((always_inline)) {
-        constexpr bool BAD = decltype(bad_tag)::value;
+      // O^T[d][row] += V^T[d][keys] P^T[keys][row], 16-key chunks.
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int mt = c >> 1, base = (c & 1) * 4;
-          const h8_t pb = as_h8(make_uint4(pw[mt][base], pw[mt][base + 1], pw[mt][base + 2], pw[mt][base + 3]));
+      for (int c = 0; c < BN / 16; ++c) {
+        const int mt = c >> 1, base = (c & 1) * 4;
+        const h8_t pb = as_h8(make_uint4(pw[mt][base], pw[mt][base + 1], pw[mt][base + 2], pw[mt][base + 3]));
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            const uint16_t *v0 = v_lds + 16 * c * D + tr_off + ((4 * dt + tr_chunk) ^ v_swizzle<D>(tr_key)) * 8;
-            uint2 lo = read_tr16(v0), hi = read_tr16(v0 + 8 * D);
-            if constexpr (BAD) {
-              lo = make_uint2(finite_part(lo.x), finite_part(lo.y));
-              hi = make_uint2(finite_part(hi.x), finite_part(hi.y));
-            }
-            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(make_uint4(lo.x, lo.y, hi.x, hi.y)), pb, o[dt], 0, 0, 0);
-          }
+        for (int dt = 0; dt < DT; ++dt) {
+          const uint16_t *v0 = v_lds + 16 * c * D + tr_off + ((4 * dt + tr_chunk) ^ v_swizzle<D>(tr_key)) * 8;
+          const uint2 lo = read_tr16(v0), hi = read_tr16(v0 + 8 * D);
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(make_uint4(lo.x, lo.y, hi.x, hi.y)), pb, o[dt], 0, 0, 0);
         }
-      };
-      bool bad = false;
-      if constexpr (MASK) bad = s_bad[ST] == it + 1;
-      if (!bad) {
-        __builtin_amdgcn_s_setprio(1);
-        pv(std::false_type{});
-        __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2 * kReadAhead, 1);
+      }
+      __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2 * kReadAhead, 1);
 #pragma unroll
-        for (int k = 0; k < 4 * DT - kReadAhead; ++k) {
-          __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 1);
-          __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2, 1);
-        }
-        __builtin_amdgcn_sched_group_barrier(kSchedMfma, kReadAhead, 1);
-        __builtin_amdgcn_s_setprio(0);
-      } else {
-        // The finite values by the products, the others added to the rows that see their
-        // key (a positive weight leaves an infinity or NaN what it is).
-        pv(std::true_type{});
-#pragma unroll 1
-        for (int key = 0; key < BN; ++key) {
-          const bool seen = key - 4 * h <= lim_lane;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              // d = 32 dt + 8 q + 4 h + e of this lane's row.
-              const int chunk = (4 * dt + q) ^ v_swizzle<D>(key);
-              const uint2 v = *reinterpret_cast<const uint2 *>(v_lds + key * D + chunk * 8 + 4 * h);
-              const uint32_t w[2] = {v.x, v.y};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint16_t x = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-                if (seen && (x & 0x7c00u) == 0x7c00u) o[dt][4 * q + e] += f16_to_f32(x);
-              }
-            }
-        }
+      for (int k = 0; k < BN / 16 * DT - kReadAhead; ++k) {
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2, 1);
+      }
+      __builtin_amdgcn_sched_group_barrier(kSchedMfma, kReadAhead, 1);
+      __builtin_amdgcn_s_setprio(0);
+      if constexpr (MASK) {
+        if (s_bad[ST] == it + 1) add_bad(j0);
       }
     }
     // Tile it + 1 (issued a tile ago) has landed in this wave's part of the other stage;
@@ -549,16 +576,25 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     if (it < t_end) step(it, std::true_type{}, S0{});
   }
 
-  float l_total = l_run + __shfl_xor(l_run, 32, 64);
+  const float l_total = l_run + __shfl_xor(l_run, 32, 64);
   const uint32_t pieces = __builtin_amdgcn_readfirstlane(pc.pieces), piece = __builtin_amdgcn_readfirstlane(pc.piece);
+  // 32 rows of each wave as f16, in a region of the idle stages.
+  auto rows_lds = [&](int v) __attribute__((always_inline)) { return (v < 2 ? k_lds_a : k_lds_b) + (v & 1) * 32 * D; };
+  static_assert(2 * 32 * D <= OUT, "output staging");
+  // d = 32 dt + 8 q + 4 h + 0 .. 3 of row n.
+  auto stage_row = [&](uint16_t *rows, int dt, int q, float a, float b2, float c, float d) __attribute__((always_inline)) {
+    const int chunk = (4 * dt + q) ^ out_swizzle<D>(n);
+    *reinterpret_cast<uint2 *>(rows + n * D + chunk * 8 + 4 * h) = make_uint2(pack_f16x2(a, b2), pack_f16x2(c, d));
+  };
+  bool join = false;
   if (pieces > 1) {
     // This piece's rows, in the accumulators' own order so that a store's lanes are
     // neighbours: per wave 8-byte slots of 64 lanes, (m, l) and then O two by two. A row
     // that saw no key here has m = -inf.
     constexpr uint32_t WAVE = packed_partial_slots(D) * 64 * 2, PIECE = 4 * WAVE;
-    float *first = p.partial + ((size_t)kvh * p.max_pieces + (rest - piece)) * PIECE + wave * WAVE + lane * 2;
+    float *tile_partial = p.partial + ((size_t)kvh * p.max_pieces + (rest - piece)) * PIECE + lane * 2;
     if (active) {
-      float *mine = first + (size_t)piece * PIECE;
+      float *mine = tile_partial + (size_t)piece * PIECE + wave * WAVE;
       store_partial2(mine, m_run, l_total);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
@@ -578,64 +614,92 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     }
     __syncthreads();
     if (s_last == 0) return;
-    // The last piece of the tile to finish joins all of them, in order.
-    if (active) {
-      float2 ml[kMostPieces];
+    // The last piece of the tile to finish joins all of them, in order: a wave takes 32
+    // values of d of 32 rows at a time (two such blocks, two pieces a round trip), of
+    // whichever wave's rows.
+    join = true;
+    const uint32_t blocks = DT * min(4u, (tokens * G - row0 + 31) / 32);
+    constexpr uint32_t FEW = 2;
+    for (uint32_t u0 = 2 * wave; u0 < blocks; u0 += 8) {
+      float acc[2][16], M[2], sum[2];
+      const float *from[2];
 #pragma unroll
-      for (uint32_t k = 0; k < kMostPieces; ++k) ml[k] = load_partial2(first + (size_t)min(k, pieces - 1) * PIECE);
-      float M = -INFINITY;
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t block = min(u0 + u, blocks - 1);
+        from[u] = tile_partial + block / DT * WAVE + (1 + 8 * (block % DT)) * 128;
+        M[u] = -INFINITY, sum[u] = 0.0f;
 #pragma unroll
-      for (uint32_t k = 0; k < kMostPieces; ++k) M = fmaxf(M, ml[k].x);
-      l_total = 0.0f;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
+        for (int r = 0; r < 16; ++r) acc[u][r] = 0.0f;
+      }
 #pragma unroll 1
-      for (uint32_t k = 0; k < pieces; ++k) {
-        const float *from = first + (size_t)k * PIECE;
-        const float2 own = load_partial2(from);
-        float2 v[8 * DT];
+      for (uint32_t s0 = 0; s0 < pieces; s0 += FEW) {
+        float2 ml[2][FEW], v[2][FEW][8];
 #pragma unroll
-        for (int i = 0; i < 8 * DT; ++i) v[i] = load_partial2(from + (1 + i) * 128);
-        if (own.x == -INFINITY) continue;
-        const float f = exp2_raw((own.x - M) * c2);
-        l_total = fmaf(own.y, f, l_total);
+        for (uint32_t k = 0; k < FEW; ++k)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+          for (int u = 0; u < 2; ++u) {
+            const float *part = from[u] + (size_t)min(s0 + k, pieces - 1) * PIECE;
+            ml[u][k] = load_partial2(part - (1 + 8 * (min(u0 + u, blocks - 1) % DT)) * 128);
 #pragma unroll
-          for (int r = 0; r < 16; r += 2) {
-            o[dt][r] = fmaf(v[8 * dt + r / 2].x, f, o[dt][r]);
-            o[dt][r + 1] = fmaf(v[8 * dt + r / 2].y, f, o[dt][r + 1]);
+            for (int i = 0; i < 8; ++i) v[u][k][i] = load_partial2(part + i * 128);
           }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float m = M[u];
+#pragma unroll
+          for (uint32_t k = 0; k < FEW; ++k) m = s0 + k < pieces ? fmaxf(m, ml[u][k].x) : m;
+          const float r = M[u] == -INFINITY ? 0.0f : exp2_raw((M[u] - m) * c2);
+          M[u] = m;
+          sum[u] *= r;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[u][i] *= r;
+#pragma unroll
+          for (uint32_t k = 0; k < FEW; ++k) {
+            // -inf: a piece in which the row saw no key.
+            const bool use = s0 + k < pieces && ml[u][k].x != -INFINITY;
+            const float f = use ? exp2_raw((ml[u][k].x - m) * c2) : 0.0f;
+            sum[u] = use ? fmaf(ml[u][k].y, f, sum[u]) : sum[u];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              acc[u][2 * i] = use ? fmaf(v[u][k][i].x, f, acc[u][2 * i]) : acc[u][2 * i];
+              acc[u][2 * i + 1] = use ? fmaf(v[u][k][i].y, f, acc[u][2 * i + 1]) : acc[u][2 * i + 1];
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t block = u0 + u;
+        if (block >= blocks) continue;
+        const float inv = 1.0f / sum[u];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          stage_row(rows_lds(block / DT), block % DT, q, acc[u][4 * q] * inv, acc[u][4 * q + 1] * inv,
+                    acc[u][4 * q + 2] * inv, acc[u][4 * q + 3] * inv);
       }
     }
   }
-  // Normalise (a row that saw no key: 0 / 0), then store through LDS: each wave writes
-  // its 32 rows as f16 into a region of the idle stages and stores them back as whole
-  // 16-byte chunks, D / 8 consecutive lanes per row.
-  const float inv = 1.0f / l_total;
+  // Normalise (a row that saw no key: 0 / 0) and store through LDS as whole 16-byte
+  // chunks, D / 8 consecutive lanes per row.
   constexpr int RPI = 64 / CPR;  // rows per store instruction
-  static_assert(2 * 32 * D <= TILE, "output staging");
-  __syncthreads();  // every wave is past its last LDS operand read
-  uint16_t *rows_lds = (wave < 2 ? k_lds_a : k_lds_b) + (wave & 1) * 32 * D;
+  if (!join) {
+    const float inv = 1.0f / l_total;
+    __syncthreads();  // every wave is past its last LDS operand read
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      uint2 v;
-      v.x = pack_f16x2(o[dt][4 * q] * inv, o[dt][4 * q + 1] * inv);
-      v.y = pack_f16x2(o[dt][4 * q + 2] * inv, o[dt][4 * q + 3] * inv);
-      const int chunk = (4 * dt + q) ^ out_swizzle<D>(n);
-      *reinterpret_cast<uint2 *>(rows_lds + n * D + chunk * 8 + 4 * h) = v;
-    }
+      for (int q = 0; q < 4; ++q)
+        stage_row(rows_lds(wave), dt, q, o[dt][4 * q] * inv, o[dt][4 * q + 1] * inv, o[dt][4 * q + 2] * inv,
+                  o[dt][4 * q + 3] * inv);
+  }
   __syncthreads();
+  const uint16_t *own_rows = rows_lds(wave);
   const int lane_o = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
   const int c_out = lane_o % CPR;
 #pragma unroll
   for (int i = 0; i < 32 / RPI; ++i) {
     const int r = i * RPI + lane_o / CPR;
-    const uint4 v = *reinterpret_cast<const uint4 *>(rows_lds + r * D + (c_out ^ out_swizzle<D>(r)) * 8);
+    const uint4 v = *reinterpret_cast<const uint4 *>(own_rows + r * D + (c_out ^ out_swizzle<D>(r)) * 8);
     const uint32_t prow = row0 + wave * 32 + r, t = prow / G, g = prow % G;
     if (t < tokens)
       *reinterpret_cast<uint4 *>(p.out + (int64_t)(range.begin + t) * p.o_tok + (int64_t)(kvh * G + g) * p.o_head +
