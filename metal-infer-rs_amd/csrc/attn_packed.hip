@@ -226,6 +226,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   constexpr int BPW = RPW / RPB;       // its direct loads of K (and V) per tile
   constexpr uint32_t GROUPS = BN / 16, HELD = 64 / GROUPS;  // 16-key groups per tile; tiles whose page ids a wave holds
   constexpr int DC = D / 16, DT = D / 32;
+  constexpr bool PIPE = D == 256;
   constexpr int TILE = BN * D, OUT = 64 * D;  // halves of a tile, and of two waves' output rows
   // One array per stage, and the stage a compile-time choice, so that the compiler can
   // tell the loads into one from the reads of the other.
@@ -353,6 +354,45 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
       load_lds16(reinterpret_cast<const uint16_t *>(ok ? vt + v_off[i] : zero), vd + i * 512);
     }
   };
+  // The same for K or V alone, where they are loaded one tile apart: V of a tile takes the
+  // page that its K has taken.
+  uint32_t page_k = 0, gone_0 = 0, gone_1 = 0, gone_2 = 0;
+  auto issue_part = [&](uint32_t ti, const uint16_t *pool, int64_t page_st, int64_t pos_st, int64_t head_st,
+                        const uint32_t (&at)[BPW], uint16_t *dst) __attribute__((always_inline)) {
+    const uint32_t key = ti * BN + wave * RPW;
+    bool there = key < kmax;
+    const uint16_t *first = pool + (int64_t)kvh * head_st;
+    if constexpr (PAGED) {
+      there = there && page_k < p.kv.pages;
+      first += (int64_t)page_k * page_st + (int64_t)(key & in_page) * pos_st;
+    } else {
+      first += (int64_t)(range.begin + key) * pos_st;
+    }
+    const char *from = reinterpret_cast<const char *>(first);
+    dst += wave * RPW * D;
+    if (there && key + RPW <= kmax) {
+#pragma unroll
+      for (int i = 0; i < BPW; ++i) load_lds16(reinterpret_cast<const uint16_t *>(from + at[i]), dst + i * 512);
+      return;
+    }
+    const char *zero = reinterpret_cast<const char *>(zero_row) + 16 * (lane % CPR);
+#pragma unroll
+    for (int i = 0; i < BPW; ++i) {
+      const bool ok = there && key + i * RPB + lane / CPR < kmax;
+      load_lds16(reinterpret_cast<const uint16_t *>(ok ? from + at[i] : zero), dst + i * 512);
+    }
+  };
+  auto issue_k = [&](uint32_t ti, int stage) __attribute__((always_inline)) {
+    if constexpr (PAGED) {
+      if (ti % HELD == 0 || ti == t_begin) load_ids(ti / HELD * HELD);
+      page_k = (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)(GROUPS * (ti % HELD) + wave * RPW / 16));
+      gone_2 = (uint32_t)(absent >> (GROUPS * (ti % HELD))) & ((1u << GROUPS) - 1);
+    }
+    issue_part(ti, p.kv.k, p.kv.k_page, p.kv.k_pos, p.kv.k_head, k_off, k_stage(stage));
+  };
+  auto issue_v = [&](uint32_t ti, int stage) __attribute__((always_inline)) {
+    issue_part(ti, p.kv.v, p.kv.v_page, p.kv.v_pos, p.kv.v_head, v_off, v_stage(stage));
+  };
   // Tiles wholly inside the first row's window need no mask.
   const uint32_t n_full = full_lim < 0 ? 0 : (uint32_t)min((int64_t)t_end, (full_lim + 1) / BN);
   // A masked tile's V may hold values that some of its rows must not see and that are
@@ -418,35 +458,46 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     }
   };
 
+  float16_t s_cur[MT];
+  auto scores = [&](const uint16_t *k_lds, float16_t (&s)[MT]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[mt][r] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < DC; ++c) {
+        const uint16_t *kp = k_lds + (32 * mt + n) * D + (((2 * c + h) ^ k_swizzle<D>(n)) * 8);
+        s[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(*reinterpret_cast<const uint4 *>(kp)), qop[c], s[mt], 0, 0, 0);
+      }
+    }
+  };
   auto step = [&](uint32_t it, auto mask_tag, auto stage_tag) __attribute__((always_inline)) {
     constexpr bool MASK = decltype(mask_tag)::value;
     constexpr int ST = decltype(stage_tag)::value;
     const uint32_t j0 = it * BN;
     const uint16_t *k_lds = ST ? k_lds_b : k_lds_a;
     const uint16_t *v_lds = ST ? v_lds_b : v_lds_a;
-    const uint32_t gone = ST ? gone_b : gone_a;
+    const uint32_t gone = PIPE ? gone_0 : ST ? gone_b : gone_a;
     if (active) {
-      // S^T[key][row]: two 32-key halves, at raised wave priority.
-      __builtin_amdgcn_s_setprio(1);
-      float16_t s[MT];
+      float16_t s[MT], nx[MT];
+      if constexpr (PIPE) {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
+        for (int mt = 0; mt < MT; ++mt) s[mt] = s_cur[mt];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[mt][r] = 0.0f;
+        for (int dt = 0; dt < DT; ++dt) asm volatile("" : "+a"(o[dt]));
+      } else {
+        // S^T[key][row]: two 32-key halves, at raised wave priority.
+        __builtin_amdgcn_s_setprio(1);
+        scores(k_lds, s);
+        __builtin_amdgcn_sched_group_barrier(kSchedDsRead, kReadAhead, 0);
 #pragma unroll
-        for (int c = 0; c < DC; ++c) {
-          const uint16_t *kp = k_lds + (32 * mt + n) * D + (((2 * c + h) ^ k_swizzle<D>(n)) * 8);
-          s[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(*reinterpret_cast<const uint4 *>(kp)), qop[c], s[mt], 0, 0, 0);
+        for (int k = 0; k < MT * DC - kReadAhead; ++k) {
+          __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
         }
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, kReadAhead, 0);
+        __builtin_amdgcn_s_setprio(0);
       }
-      __builtin_amdgcn_sched_group_barrier(kSchedDsRead, kReadAhead, 0);
-#pragma unroll
-      for (int k = 0; k < MT * DC - kReadAhead; ++k) {
-        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(kSchedMfma, kReadAhead, 0);
-      __builtin_amdgcn_s_setprio(0);
       // Key 32 mt + 8 (r >> 2) + 4 h + (r & 3) of the tile is seen when it is at most
       // lim_rel; the lane's 4 h moves to the limit, so each compare is with a constant.
       int lim_lane = BN;
@@ -485,7 +536,45 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
       };
       // The reference moves only when a weight leaves f16's range: the sum is then +inf
       // or NaN, as it is for a row without a reference yet (m_run = -inf).
-      weights(m_run * c2 - kBias);
+      constexpr int AHEAD = 4;
+      uint4 kf[AHEAD], vf[AHEAD];
+      auto read_k = [&](int c) __attribute__((always_inline)) {
+        kf[c % AHEAD] = *reinterpret_cast<const uint4 *>((ST ? k_lds_a : k_lds_b) + n * D + (((2 * c + h) ^ k_swizzle<D>(n)) * 8));
+      };
+      auto read_v = [&](int i) __attribute__((always_inline)) {
+        const uint16_t *v0 = v_lds + 16 * (i / DT) * D + tr_off + ((4 * (i % DT) + tr_chunk) ^ v_swizzle<D>(tr_key)) * 8;
+        const uint2 lo = read_tr16(v0), hi = read_tr16(v0 + 8 * D);
+        vf[i % AHEAD] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      };
+      if constexpr (PIPE) {
+        // The next tile's scores beside this one's softmax (of the last tile: of whatever the
+        // stage holds, and not used), each operand read AHEAD of its product; the order is
+        // the source's.
+        const float mc = m_run * c2 - kBias;
+        float ps0 = 0.0f, ps1 = 0.0f, even = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) nx[0][r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < AHEAD; ++c) read_k(c);
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+          __builtin_amdgcn_sched_barrier(0);
+          nx[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(kf[c % AHEAD]), qop[c], nx[0], 0, 0, 0);
+          if (c + AHEAD < DC) read_k(c + AHEAD);
+          else read_v(c + AHEAD - DC);
+          const float e = exp2_raw(fmaf(s[0][c], c2, -mc));
+          if (c & 1) {
+            pw[0][c >> 1] = pack_f16x2(even, e);
+            if (c & 2) ps1 = dot2(pw[0][c >> 1], 0x3c003c00u, ps1);
+            else ps0 = dot2(pw[0][c >> 1], 0x3c003c00u, ps0);
+          }
+          even = e;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        psum = ps0 + ps1;
+      } else {
+        weights(m_run * c2 - kBias);
+      }
       if (__any(!(psum <= __FLT_MAX__))) {
         float mx = -INFINITY;
 #pragma unroll
@@ -506,28 +595,44 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
       }
       l_run += psum;
       // O^T[d][row] += V^T[d][keys] P^T[keys][row], 16-key chunks.
-      __builtin_amdgcn_s_setprio(1);
+      if constexpr (PIPE) {
 #pragma unroll
-      for (int c = 0; c < BN / 16; ++c) {
-        const int mt = c >> 1, base = (c & 1) * 4;
-        const h8_t pb = as_h8(make_uint4(pw[mt][base], pw[mt][base + 1], pw[mt][base + 2], pw[mt][base + 3]));
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const uint16_t *v0 = v_lds + 16 * c * D + tr_off + ((4 * dt + tr_chunk) ^ v_swizzle<D>(tr_key)) * 8;
-          const uint2 lo = read_tr16(v0), hi = read_tr16(v0 + 8 * D);
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(make_uint4(lo.x, lo.y, hi.x, hi.y)), pb, o[dt], 0, 0, 0);
+        for (int i = 0; i < 2 * DT; ++i) {
+          const int base = i / DT * 4;
+          const h8_t pb = as_h8(make_uint4(pw[0][base], pw[0][base + 1], pw[0][base + 2], pw[0][base + 3]));
+          __builtin_amdgcn_sched_barrier(0);
+          o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(vf[i % AHEAD]), pb, o[i % DT], 0, 0, 0);
+          if (i + AHEAD < 2 * DT) read_v(i + AHEAD);
         }
-      }
-      __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2 * kReadAhead, 1);
+        __builtin_amdgcn_sched_barrier(0);
+      } else {
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int k = 0; k < BN / 16 * DT - kReadAhead; ++k) {
-        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 1);
-        __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2, 1);
+        for (int c = 0; c < BN / 16; ++c) {
+          const int mt = c >> 1, base = (c & 1) * 4;
+          const h8_t pb = as_h8(make_uint4(pw[mt][base], pw[mt][base + 1], pw[mt][base + 2], pw[mt][base + 3]));
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            const uint16_t *v0 = v_lds + 16 * c * D + tr_off + ((4 * dt + tr_chunk) ^ v_swizzle<D>(tr_key)) * 8;
+            const uint2 lo = read_tr16(v0), hi = read_tr16(v0 + 8 * D);
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(make_uint4(lo.x, lo.y, hi.x, hi.y)), pb, o[dt], 0, 0, 0);
+          }
+        }
+        __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2 * kReadAhead, 1);
+#pragma unroll
+        for (int k = 0; k < BN / 16 * DT - kReadAhead; ++k) {
+          __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 1);
+          __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2, 1);
+        }
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, kReadAhead, 1);
+        __builtin_amdgcn_s_setprio(0);
       }
-      __builtin_amdgcn_sched_group_barrier(kSchedMfma, kReadAhead, 1);
-      __builtin_amdgcn_s_setprio(0);
       if constexpr (MASK) {
         if (s_bad[ST] == it + 1) add_bad(j0);
+      }
+      if constexpr (PIPE) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) s_cur[mt] = nx[mt];
       }
     }
     // Tile it + 1 (issued a tile ago) has landed in this wave's part of the other stage;
@@ -535,7 +640,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     wait_vmcnt<0>();
     if (it + 1 < t_end) look(it + 1, ST ^ 1);
     __syncthreads();
-    if (it + 2 < t_end) issue_tile(it + 2, ST);
+    if constexpr (PIPE) {
+      gone_0 = gone_1, gone_1 = gone_2;
+      if (it + 2 < t_end) issue_v(it + 2, ST);
+      if (it + 3 < t_end) issue_k(it + 3, ST ^ 1);
+    } else {
+      if (it + 2 < t_end) issue_tile(it + 2, ST);
+    }
   };
 
   if (t_begin < t_end) {
@@ -545,15 +656,32 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     // Loads complete in issue order, so vmcnt(2 BPW) leaves only the second tile's pending.
     // The barrier is a bare s_barrier (a workgroup fence would wait for every load); each
     // wave has waited for its own part, and the memory clobber keeps LDS reads below it.
-    issue_tile(t_begin, 0);
-    if (t_begin + 1 < t_end) {
-      issue_tile(t_begin + 1, 1);
-      wait_vmcnt<2 * BPW>();
-    } else {
+    if constexpr (PIPE) {
+      issue_k(t_begin, 0);
+      gone_0 = gone_2;
+      issue_v(t_begin, 0);
+      if (t_begin + 1 < t_end) {
+        issue_k(t_begin + 1, 1);
+        gone_1 = gone_2;
+      }
       wait_vmcnt<0>();
+      look(t_begin, 0);
+      __syncthreads();
+      if (active) scores(k_lds_a, s_cur);
+      __syncthreads();
+      if (t_begin + 1 < t_end) issue_v(t_begin + 1, 1);
+      if (t_begin + 2 < t_end) issue_k(t_begin + 2, 0);
+    } else {
+      issue_tile(t_begin, 0);
+      if (t_begin + 1 < t_end) {
+        issue_tile(t_begin + 1, 1);
+        wait_vmcnt<2 * BPW>();
+      } else {
+        wait_vmcnt<0>();
+      }
+      look(t_begin, 0);
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
-    look(t_begin, 0);
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     using S0 = std::integral_constant<int, 0>;
     using S1 = std::integral_constant<int, 1>;
     uint32_t it = t_begin;
