@@ -309,9 +309,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     }
   };
 
-  // Direct loads of tile ti into a stage: each wave fills 16 rows, lane L writing bytes
-  // 16 L .. 16 L + 15 of a 1 KB block, so it fetches the 16 bytes that belong at that
-  // swizzled position. A scalar base and loop-invariant offsets.
+  // Direct loads of tile ti's K or V into a stage: each wave fills RPW rows, lane L writing
+  // bytes 16 L .. 16 L + 15 of a 1 KB block, so it fetches the 16 bytes that belong at that
+  // swizzled position. A scalar base and loop-invariant offsets; rows past the last key
+  // that any row sees, or without a page, take an offset past the buffer's end, which
+  // loads zeros. (Buffer loads without branches: the compiler then counts exactly which
+  // loads into LDS are in flight, and waits for no others.)
   uint32_t k_off[BPW], v_off[BPW];
 #pragma unroll
   for (int i = 0; i < BPW; ++i) {
@@ -319,79 +322,42 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     k_off[i] = ((uint32_t)r * (uint32_t)p.kv.k_pos + ((pc ^ k_swizzle<D>(row)) * 8)) * 2u;
     v_off[i] = ((uint32_t)r * (uint32_t)p.kv.v_pos + ((pc ^ v_swizzle<D>(row)) * 8)) * 2u;
   }
-  auto issue_tile = [&](uint32_t ti, int stage) __attribute__((always_inline)) {
-    if (PAGED && (ti % HELD == 0 || ti == t_begin)) load_ids(ti / HELD * HELD);
-    const uint32_t key = ti * BN + wave * RPW;
-    const char *kt, *vt;
-    bool there = key < kmax;
+  uint32_t page_of = 0, gone_new = 0;  // of the tile found last: its page, and its groups without one
+  auto find = [&](uint32_t ti) __attribute__((always_inline)) {
     if constexpr (PAGED) {
-      const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)(GROUPS * (ti % HELD) + wave * RPW / 16));
-      there = there && page < p.kv.pages;
-      (stage ? gone_b : gone_a) = (uint32_t)(absent >> (GROUPS * (ti % HELD))) & ((1u << GROUPS) - 1);
-      kt = reinterpret_cast<const char *>(p.kv.k + (int64_t)page * p.kv.k_page + (int64_t)(key & in_page) * p.kv.k_pos +
-                                          (int64_t)kvh * p.kv.k_head);
-      vt = reinterpret_cast<const char *>(p.kv.v + (int64_t)page * p.kv.v_page + (int64_t)(key & in_page) * p.kv.v_pos +
-                                          (int64_t)kvh * p.kv.v_head);
-    } else {
-      kt = reinterpret_cast<const char *>(p.kv.k + (int64_t)(range.begin + key) * p.kv.k_pos + (int64_t)kvh * p.kv.k_head);
-      vt = reinterpret_cast<const char *>(p.kv.v + (int64_t)(range.begin + key) * p.kv.v_pos + (int64_t)kvh * p.kv.v_head);
-    }
-    uint16_t *kd = k_stage(stage) + wave * RPW * D, *vd = v_stage(stage) + wave * RPW * D;
-    if (there && key + RPW <= kmax) {
-#pragma unroll
-      for (int i = 0; i < BPW; ++i) {
-        load_lds16(reinterpret_cast<const uint16_t *>(kt + k_off[i]), kd + i * 512);
-        load_lds16(reinterpret_cast<const uint16_t *>(vt + v_off[i]), vd + i * 512);
-      }
-      return;
-    }
-    // Rows past the last key that any row sees, or without a page, are zeros.
-    const char *zero = reinterpret_cast<const char *>(zero_row) + 16 * (lane % CPR);
-#pragma unroll
-    for (int i = 0; i < BPW; ++i) {
-      const bool ok = there && key + i * RPB + lane / CPR < kmax;
-      load_lds16(reinterpret_cast<const uint16_t *>(ok ? kt + k_off[i] : zero), kd + i * 512);
-      load_lds16(reinterpret_cast<const uint16_t *>(ok ? vt + v_off[i] : zero), vd + i * 512);
+      if (ti % HELD == 0 || ti == t_begin) load_ids(ti / HELD * HELD);
+      page_of = (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)(GROUPS * (ti % HELD) + wave * RPW / 16));
+      gone_new = (uint32_t)(absent >> (GROUPS * (ti % HELD))) & ((1u << GROUPS) - 1);
     }
   };
-  // The same for K or V alone, where they are loaded one tile apart: V of a tile takes the
-  // page that its K has taken.
-  uint32_t page_k = 0, gone_0 = 0, gone_1 = 0, gone_2 = 0;
-  auto issue_part = [&](uint32_t ti, const uint16_t *pool, int64_t page_st, int64_t pos_st, int64_t head_st,
-                        const uint32_t (&at)[BPW], uint16_t *dst) __attribute__((always_inline)) {
+  auto issue = [&](uint32_t ti, const uint16_t *pool, int64_t page_st, int64_t pos_st, int64_t head_st,
+                   const uint32_t (&at)[BPW], uint16_t *dst) __attribute__((always_inline)) {
     const uint32_t key = ti * BN + wave * RPW;
-    bool there = key < kmax;
+    uint32_t rows = key < kmax ? kmax - key : 0;
     const uint16_t *first = pool + (int64_t)kvh * head_st;
     if constexpr (PAGED) {
-      there = there && page_k < p.kv.pages;
-      first += (int64_t)page_k * page_st + (int64_t)(key & in_page) * pos_st;
+      rows = page_of < p.kv.pages ? rows : 0;
+      first += (int64_t)page_of * page_st + (int64_t)(key & in_page) * pos_st;
     } else {
       first += (int64_t)(range.begin + key) * pos_st;
     }
-    const char *from = reinterpret_cast<const char *>(first);
-    dst += wave * RPW * D;
-    if (there && key + RPW <= kmax) {
-#pragma unroll
-      for (int i = 0; i < BPW; ++i) load_lds16(reinterpret_cast<const uint16_t *>(from + at[i]), dst + i * 512);
-      return;
-    }
-    const char *zero = reinterpret_cast<const char *>(zero_row) + 16 * (lane % CPR);
 #pragma unroll
     for (int i = 0; i < BPW; ++i) {
-      const bool ok = there && key + i * RPB + lane / CPR < kmax;
-      load_lds16(reinterpret_cast<const uint16_t *>(ok ? from + at[i] : zero), dst + i * 512);
+      const bool ok = i * RPB + lane / CPR < rows;
+      load_lds16_buffer(first, ok ? at[i] : kBufferEnd, dst + wave * RPW * D + i * 512);
     }
   };
   auto issue_k = [&](uint32_t ti, int stage) __attribute__((always_inline)) {
-    if constexpr (PAGED) {
-      if (ti % HELD == 0 || ti == t_begin) load_ids(ti / HELD * HELD);
-      page_k = (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)(GROUPS * (ti % HELD) + wave * RPW / 16));
-      gone_2 = (uint32_t)(absent >> (GROUPS * (ti % HELD))) & ((1u << GROUPS) - 1);
-    }
-    issue_part(ti, p.kv.k, p.kv.k_page, p.kv.k_pos, p.kv.k_head, k_off, k_stage(stage));
+    issue(ti, p.kv.k, p.kv.k_page, p.kv.k_pos, p.kv.k_head, k_off, k_stage(stage));
   };
   auto issue_v = [&](uint32_t ti, int stage) __attribute__((always_inline)) {
-    issue_part(ti, p.kv.v, p.kv.v_page, p.kv.v_pos, p.kv.v_head, v_off, v_stage(stage));
+    issue(ti, p.kv.v, p.kv.v_page, p.kv.v_pos, p.kv.v_head, v_off, v_stage(stage));
+  };
+  auto issue_tile = [&](uint32_t ti, int stage) __attribute__((always_inline)) {
+    find(ti);
+    (stage ? gone_b : gone_a) = gone_new;
+    issue_k(ti, stage);
+    issue_v(ti, stage);
   };
   // Tiles wholly inside the first row's window need no mask.
   const uint32_t n_full = full_lim < 0 ? 0 : (uint32_t)min((int64_t)t_end, (full_lim + 1) / BN);
@@ -477,7 +443,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     const uint32_t j0 = it * BN;
     const uint16_t *k_lds = ST ? k_lds_b : k_lds_a;
     const uint16_t *v_lds = ST ? v_lds_b : v_lds_a;
-    const uint32_t gone = PIPE ? gone_0 : ST ? gone_b : gone_a;
+    const uint32_t gone = !PIPE && ST ? gone_b : gone_a;
+    // Issued here and not at the end of the step before, where the loads would be in flight
+    // over the loop's back edge: the compiler then takes one stage's for the other's, and
+    // waits for them before it reads the stage that is complete.
+    if (!PIPE && it + 1 < t_end) issue_tile(it + 1, ST ^ 1);
     if (active) {
       float16_t s[MT], nx[MT];
       if constexpr (PIPE) {
@@ -635,34 +605,34 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
         for (int mt = 0; mt < MT; ++mt) s_cur[mt] = nx[mt];
       }
     }
-    // Tile it + 1 (issued a tile ago) has landed in this wave's part of the other stage;
-    // after the barrier nobody reads this stage, which then receives tile it + 2.
+    // Tile it + 1 has landed in this wave's part of the other stage; after the barrier
+    // nobody reads this stage, which then receives tile it + 2 (with PIPE its V, and the K
+    // of tile it + 3 goes into the other stage).
     wait_vmcnt<0>();
     if (it + 1 < t_end) look(it + 1, ST ^ 1);
     __syncthreads();
     if constexpr (PIPE) {
-      gone_0 = gone_1, gone_1 = gone_2;
+      gone_a = gone_b, gone_b = gone_new;
       if (it + 2 < t_end) issue_v(it + 2, ST);
-      if (it + 3 < t_end) issue_k(it + 3, ST ^ 1);
-    } else {
-      if (it + 2 < t_end) issue_tile(it + 2, ST);
+      if (it + 3 < t_end) {
+        find(it + 3);
+        issue_k(it + 3, ST ^ 1);
+      }
     }
   };
 
   if (t_begin < t_end) {
     if (tid < 2) s_bad[tid] = 0;
     __syncthreads();
-    // The first tile (stage 0) is computed once it has landed; the second stays in flight.
-    // Loads complete in issue order, so vmcnt(2 BPW) leaves only the second tile's pending.
-    // The barrier is a bare s_barrier (a workgroup fence would wait for every load); each
-    // wave has waited for its own part, and the memory clobber keeps LDS reads below it.
     if constexpr (PIPE) {
+      find(t_begin);
+      gone_a = gone_new;
       issue_k(t_begin, 0);
-      gone_0 = gone_2;
       issue_v(t_begin, 0);
       if (t_begin + 1 < t_end) {
+        find(t_begin + 1);
+        gone_b = gone_new;
         issue_k(t_begin + 1, 1);
-        gone_1 = gone_2;
       }
       wait_vmcnt<0>();
       look(t_begin, 0);
@@ -670,17 +640,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
       if (active) scores(k_lds_a, s_cur);
       __syncthreads();
       if (t_begin + 1 < t_end) issue_v(t_begin + 1, 1);
-      if (t_begin + 2 < t_end) issue_k(t_begin + 2, 0);
+      if (t_begin + 2 < t_end) {
+        find(t_begin + 2);
+        issue_k(t_begin + 2, 0);
+      }
     } else {
       issue_tile(t_begin, 0);
-      if (t_begin + 1 < t_end) {
-        issue_tile(t_begin + 1, 1);
-        wait_vmcnt<2 * BPW>();
-      } else {
-        wait_vmcnt<0>();
-      }
+      wait_vmcnt<0>();
       look(t_begin, 0);
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      __syncthreads();
     }
     using S0 = std::integral_constant<int, 0>;
     using S1 = std::integral_constant<int, 1>;

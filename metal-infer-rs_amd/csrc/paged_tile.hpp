@@ -71,6 +71,16 @@ __device__ __forceinline__ void wait_vmcnt() {
   __builtin_amdgcn_s_waitcnt(kWaitVmcnt0 | (N & 15) | ((N >> 4) << 14));
 }
 
+// A direct global -> LDS load of 16 bytes per lane, as load_lds16, from the uniform address
+// `base` plus a byte offset per lane; an offset of kBufferEnd or more loads zeros.
+constexpr uint32_t kBufferEnd = 0x80000000u;
+__device__ __forceinline__ void load_lds16_buffer(const uint16_t *base, uint32_t offset, uint16_t *lds) {
+  // Raw 32-bit data, no stride, no swizzle.
+  const __amdgpu_buffer_rsrc_t r =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(base), 0, (int)kBufferEnd, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) uint16_t *)lds, 16, (int)offset, 0, 0, 0);
+}
+
 // s_waitcnt lgkmcnt(0): the wave's LDS accesses are done.
 __device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xC07F); }
 
