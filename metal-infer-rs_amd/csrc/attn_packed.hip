@@ -40,7 +40,12 @@ constexpr int BM = kPrefillBlockM;  // rows per workgroup
 // reference's (a long tail of them counts); it cancels against the row sum.
 constexpr float kBias = 8.0f;
 // Fewest key tiles of a piece of a cut row tile, and most pieces.
-constexpr uint32_t kLeastPiece = 4, kMostPieces = 16;
+constexpr uint32_t kLeastPiece = 4, kMostPieces = 32;
+// More pieces than kOneJoin are joined a few at a time by several workgroups, and then those
+// joins: about the square root of their number. (64 rows of 64 heads on 4000 keys, 16 pieces
+// a tile: 48 us by one workgroup each, 42 us four at a time.)
+constexpr uint32_t kOneJoin = 8;
+__device__ __forceinline__ uint32_t join_size(uint32_t pieces) { return pieces > 16 ? 6 : 4; }
 constexpr int kReadAhead = 4;       // LDS operand reads in flight ahead of the MFMAs
 constexpr int kSchedMfma = 0x008, kSchedDsRead = 0x100;
 
@@ -685,8 +690,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   bool join = false;
   if (pieces > 1) {
     // This piece's rows, in the accumulators' own order so that a store's lanes are
-    // neighbours: per wave 8-byte slots of 64 lanes, (m, l) and then O two by two. A row
-    // that saw no key here has m = -inf.
+    // neighbours: per wave 8-byte slots of 64 lanes, (m, l), room for those of a
+    // join, and O two by two. A row that saw no key here has m = -inf.
     constexpr uint32_t WAVE = packed_partial_slots(D) * 64 * 2, PIECE = 4 * WAVE;
     float *tile_partial = p.partial + ((size_t)kvh * p.max_pieces + (rest - piece)) * PIECE + lane * 2;
     if (active) {
@@ -695,84 +700,107 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int r = 0; r < 16; r += 2) store_partial2(mine + (1 + 8 * dt + r / 2) * 128, o[dt][r], o[dt][r + 1]);
+        for (int r = 0; r < 16; r += 2) store_partial2(mine + (2 + 8 * dt + r / 2) * 128, o[dt][r], o[dt][r + 1]);
     }
-    wait_vmcnt<0>();
-    __syncthreads();
-    if (tid == 0) {
-      uint32_t *counter = p.counters + (size_t)(kvh * p.max_pieces + pc.cut) * p.counter_stride;
-      const bool last = arrive(counter) == pieces - 1;
-      if (last) {
-        acquire_partials();
-        __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-      s_last = last;
-    }
-    __syncthreads();
-    if (s_last == 0) return;
-    // The last piece of the tile to finish joins all of them, in order: a wave takes 32
-    // values of d of 32 rows at a time (two such blocks, two pieces a round trip), of
-    // whichever wave's rows.
+    // The last of a tile's pieces to finish joins all of them, in order; of more than
+    // kOneJoin, the last of each few in a row joins those, into the first of them, and the
+    // last of these joins does the rest. A wave takes 32 values of d of 32 rows at a time
+    // (two such blocks, two pieces a round trip), of whichever wave's rows.
     join = true;
+    const bool steps = pieces > kOneJoin;
+    const uint32_t few = join_size(pieces);
+    uint32_t first = steps ? piece / few * few : 0, parts = steps ? min(pieces - first, few) : pieces, gap = 1;
+    uint32_t counter_at = steps ? p.max_pieces * (p.kv_heads + kvh) + (rest - piece) + first : kvh * p.max_pieces + pc.cut;
+    counter_at = __builtin_amdgcn_readfirstlane(counter_at);
     const uint32_t blocks = DT * min(4u, (tokens * G - row0 + 31) / 32);
-    constexpr uint32_t FEW = 2;
-    for (uint32_t u0 = 2 * wave; u0 < blocks; u0 += 8) {
-      float acc[2][16], M[2], sum[2];
-      const float *from[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t block = min(u0 + u, blocks - 1);
-        from[u] = tile_partial + block / DT * WAVE + (1 + 8 * (block % DT)) * 128;
-        M[u] = -INFINITY, sum[u] = 0.0f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[u][r] = 0.0f;
-      }
 #pragma unroll 1
-      for (uint32_t s0 = 0; s0 < pieces; s0 += FEW) {
-        float2 ml[2][FEW], v[2][FEW][8];
-#pragma unroll
-        for (uint32_t k = 0; k < FEW; ++k)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float *part = from[u] + (size_t)min(s0 + k, pieces - 1) * PIECE;
-            ml[u][k] = load_partial2(part - (1 + 8 * (min(u0 + u, blocks - 1) % DT)) * 128);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[u][k][i] = load_partial2(part + i * 128);
-          }
+    for (;;) {
+      wait_vmcnt<0>();
+      __syncthreads();
+      if (tid == 0) {
+        uint32_t *counter = p.counters + (size_t)counter_at * p.counter_stride;
+        const bool last = arrive(counter) == parts - 1;
+        if (last) {
+          acquire_partials();
+          __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        s_last = last;
+      }
+      __syncthreads();
+      if (s_last == 0) return;
+      const bool final = !steps || gap != 1;
+      constexpr uint32_t FEW = 2;
+      for (uint32_t u0 = 2 * wave; u0 < blocks; u0 += 8) {
+        float acc[2][16], M[2], sum[2];
+        float *from[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          float m = M[u];
+          const uint32_t block = min(u0 + u, blocks - 1);
+          from[u] = tile_partial + (size_t)first * PIECE + block / DT * WAVE + (2 + 8 * (block % DT)) * 128;
+          M[u] = -INFINITY, sum[u] = 0.0f;
 #pragma unroll
-          for (uint32_t k = 0; k < FEW; ++k) m = s0 + k < pieces ? fmaxf(m, ml[u][k].x) : m;
-          const float r = M[u] == -INFINITY ? 0.0f : exp2_raw((M[u] - m) * c2);
-          M[u] = m;
-          sum[u] *= r;
+          for (int r = 0; r < 16; ++r) acc[u][r] = 0.0f;
+        }
+        // A piece's (m, l) are in its first slot, those of a join in the second.
+        auto ml_at = [&](int u) __attribute__((always_inline)) {
+          return (gap == 1 ? 2 : 1) * 128 + 8 * (min(u0 + u, blocks - 1) % DT) * 128;
+        };
+#pragma unroll 1
+        for (uint32_t s0 = 0; s0 < parts; s0 += FEW) {
+          float2 ml[2][FEW], v[2][FEW][8];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[u][i] *= r;
+          for (uint32_t k = 0; k < FEW; ++k)
 #pragma unroll
-          for (uint32_t k = 0; k < FEW; ++k) {
-            // -inf: a piece in which the row saw no key.
-            const bool use = s0 + k < pieces && ml[u][k].x != -INFINITY;
-            const float f = use ? exp2_raw((ml[u][k].x - m) * c2) : 0.0f;
-            sum[u] = use ? fmaf(ml[u][k].y, f, sum[u]) : sum[u];
+            for (int u = 0; u < 2; ++u) {
+              const float *part = from[u] + (size_t)(min(s0 + k, parts - 1) * gap) * PIECE;
+              ml[u][k] = load_partial2(part - ml_at(u));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              acc[u][2 * i] = use ? fmaf(v[u][k][i].x, f, acc[u][2 * i]) : acc[u][2 * i];
-              acc[u][2 * i + 1] = use ? fmaf(v[u][k][i].y, f, acc[u][2 * i + 1]) : acc[u][2 * i + 1];
+              for (int i = 0; i < 8; ++i) v[u][k][i] = load_partial2(part + i * 128);
+            }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float m = M[u];
+#pragma unroll
+            for (uint32_t k = 0; k < FEW; ++k) m = s0 + k < parts ? fmaxf(m, ml[u][k].x) : m;
+            const float r = M[u] == -INFINITY ? 0.0f : exp2_raw((M[u] - m) * c2);
+            M[u] = m;
+            sum[u] *= r;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[u][i] *= r;
+#pragma unroll
+            for (uint32_t k = 0; k < FEW; ++k) {
+              // -inf: a piece in which the row saw no key.
+              const bool use = s0 + k < parts && ml[u][k].x != -INFINITY;
+              const float f = use ? exp2_raw((ml[u][k].x - m) * c2) : 0.0f;
+              sum[u] = use ? fmaf(ml[u][k].y, f, sum[u]) : sum[u];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                acc[u][2 * i] = use ? fmaf(v[u][k][i].x, f, acc[u][2 * i]) : acc[u][2 * i];
+                acc[u][2 * i + 1] = use ? fmaf(v[u][k][i].y, f, acc[u][2 * i + 1]) : acc[u][2 * i + 1];
+              }
             }
           }
         }
-      }
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t block = u0 + u;
-        if (block >= blocks) continue;
-        const float inv = 1.0f / sum[u];
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t block = u0 + u;
+          if (block >= blocks) continue;
+          if (final) {
+            const float inv = 1.0f / sum[u];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          stage_row(rows_lds(block / DT), block % DT, q, acc[u][4 * q] * inv, acc[u][4 * q + 1] * inv,
-                    acc[u][4 * q + 2] * inv, acc[u][4 * q + 3] * inv);
+            for (int q = 0; q < 4; ++q)
+              stage_row(rows_lds(block / DT), block % DT, q, acc[u][4 * q] * inv, acc[u][4 * q + 1] * inv,
+                        acc[u][4 * q + 2] * inv, acc[u][4 * q + 3] * inv);
+          } else {
+            if (block % DT == 0) store_partial2(from[u] - 128, M[u], sum[u]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) store_partial2(from[u] + i * 128, acc[u][2 * i], acc[u][2 * i + 1]);
+          }
+        }
       }
+      if (final) break;
+      first = 0, parts = (pieces + few - 1) / few, gap = few;
+      counter_at = __builtin_amdgcn_readfirstlane(kvh * p.max_pieces + pc.cut);
     }
   }
   // Normalise (a row that saw no key: 0 / 0) and store through LDS as whole 16-byte

@@ -406,17 +406,17 @@ struct PackedParams {
   float scale_log2;
   // Row tiles with more than an even share of the keys are cut into pieces: at most
   // max_pieces of them per KV head (0: none), whose rows go to `partial`
-  // (packed_partial_floats), one counter per cut tile (max_pieces per KV head, zero between
-  // kernels, counter_stride words apart). share: workgroups of a KV head that the chip
-  // runs at once.
+  // (packed_partial_floats), a counter per cut tile and one per piece (2 max_pieces per KV
+  // head, zero between kernels, counter_stride words apart). share: workgroups of a KV head
+  // that the chip runs at once.
   uint32_t max_pieces, share;
   float *partial;
   uint32_t *counters;
   uint32_t counter_stride;
 };
 constexpr uint32_t kPackedMaxBatch = 512;  // sequences a launch
-// 8-byte slots per lane of a piece's wave: (m, l), then O two values a slot.
-constexpr uint32_t packed_partial_slots(uint32_t head_dim) { return 1 + head_dim / 4; }
+// 8-byte slots per lane of a piece's wave: (m, l), those of a join, O two values a slot.
+constexpr uint32_t packed_partial_slots(uint32_t head_dim) { return 2 + head_dim / 4; }
 constexpr uint64_t packed_partial_floats(uint64_t pieces, uint64_t kv_heads, uint32_t head_dim) {
   return pieces * kv_heads * 4 * packed_partial_slots(head_dim) * 64 * 2;
 }

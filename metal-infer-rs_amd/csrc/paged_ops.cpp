@@ -226,9 +226,9 @@ mi_status packed(mi_batch *batch, const mi_tensor *q, const mi_tensor *key, cons
   // Twice the workgroups that run at once: an even share each, and a last piece per tile.
   Context *ctx = batch->ctx;
   p.share = std::max(1u, kernels::packed_workgroups(ctx->compute_units, config->head_dim) / p.kv_heads);
-  p.max_pieces = (uint64_t)2 * p.share * p.kv_heads <= ctx->split_counter_count ? 2 * p.share : 0;
+  p.max_pieces = (uint64_t)4 * p.share * p.kv_heads <= ctx->split_counter_count ? 2 * p.share : 0;
   p.counters = ctx->split_counters;
-  p.counter_stride = kernels::counter_stride((uint64_t)p.max_pieces * p.kv_heads, ctx->split_counter_count);
+  p.counter_stride = kernels::counter_stride((uint64_t)2 * p.max_pieces * p.kv_heads, ctx->split_counter_count);
   void *scratch = nullptr;
   if (p.max_pieces != 0) {
     const uint64_t floats = kernels::packed_partial_floats(p.max_pieces, p.kv_heads, config->head_dim);
