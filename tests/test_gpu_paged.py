@@ -721,3 +721,134 @@ def test_nothing_to_do(ctx):
     finally:
         ctx.set_kernel_profiling(False)
     assert (ctx.download(out) == 0x4321).all()
+
+
+# ------------------------------------------------------- how the work is shared --
+
+@pytest.mark.parametrize("hq,hkv,d,size,batch", [(16, 8, 128, 16, 20), (8, 8, 64, 32, 24), (4, 4, 32, 16, 40),
+                                                 (8, 4, 256, 64, 33)])
+def test_decode_of_many_units(ctx, hq, hkv, d, size, batch):
+    """Enough (sequence, KV head) units that each wave walks a share of all tiles: shares that
+    end inside a unit, units of one tile, of none, and one that many waves share."""
+    rng = np.random.default_rng(61)
+    lengths = [int(n) for n in rng.integers(0, 400, batch)]
+    lengths[3], lengths[4], lengths[5], lengths[-1] = 2900, 0, 1, 0
+    missing = [(3, p) for p in range(5, 2900 // size, 3)]
+    cache = Cache(ctx, rng, lengths, -(-2900 // size), size, hkv, d, missing=missing)
+    q = (1.5 * rng.standard_normal((batch, hq, d))).astype(np.float16)
+    got = decode(ctx, cache, q, hq)
+    hold(got, *decode_want(cache, q), f"decode {batch} x {hkv}")
+    assert np.array_equal(got, decode(ctx, cache, q, hq)), "two calls differ"
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("hq,hkv,d", [(2, 1, 128), (4, 4, 64), (3, 1, 256)])
+def test_packed_one_long_prompt_among_many(ctx, hq, hkv, d, causal):
+    """More sequences than lanes, most of them empty or short, and two whose row tiles are cut."""
+    rng = np.random.default_rng(62)
+    counts = [int(n) for n in rng.integers(0, 4, 150)]
+    counts[70], counts[149] = 1100, 600
+    starts = starts_of(counts)
+    n = int(starts[-1])
+    q, k, v = (rng.standard_normal((n, h, d)).astype(np.float16) for h in (hq, hkv, hkv))
+    batch = ctx.begin_batch()
+    out = batch.attention_packed(*[ctx.tensor(x.view(np.uint16)) for x in (q, k, v)], ctx.tensor(starts, U32),
+                                 AttentionConfig(hq, hkv, d, causal))
+    batch.finish()
+    hold(ctx.download(out), *packed_want(q, k, v, starts, causal))
+
+
+@pytest.mark.parametrize("d,size", [(128, 16), (64, 32), (32, 16), (256, 16)])
+@pytest.mark.parametrize("keys", [1100, 2500, 6000, 20000])
+def test_paged_few_rows_on_a_long_cache(ctx, keys, d, size):
+    """One row tile in up to 32 pieces, joined at once or in two steps, some of which see no
+    key; the same when captured and replayed."""
+    rng = np.random.default_rng(keys + d)
+    pages = -(-keys // size)
+    missing = [(0, p) for p in range(pages // 3, pages // 2)]
+    cache = Cache(ctx, rng, [keys, 7], pages, size, 1, d, missing=missing)
+    starts = starts_of([9, 2])
+    q = rng.standard_normal((11, 5, d)).astype(np.float16)
+    got = paged(ctx, cache, q, starts, 5)
+    hold(got, *paged_want(cache, q, starts, True))
+    t, s, out = ctx.tensor(q.view(np.uint16)), ctx.tensor(starts, U32), ctx.empty(q.shape)
+    batch = ctx.begin_capture()
+    batch.attention_paged(t, cache.key_pages, cache.value_pages, cache.device_table, cache.device_lengths, s,
+                          AttentionConfig(5, 1, d), out=out)
+    graph = batch.end_capture()
+    for _ in range(3):
+        ctx.upload(out, np.zeros(q.shape, np.uint16))
+        graph.launch()
+        ctx.synchronize()
+        assert np.array_equal(ctx.download(out), got)
+        assert np.array_equal(paged(ctx, cache, q, starts, 5), got)
+    graph.destroy()
+
+
+def test_more_sequences_than_one_launch_takes(ctx):
+    rng = np.random.default_rng(63)
+    hq, hkv, d, b = 2, 1, 64, 1100
+    counts = [int(n) for n in rng.integers(0, 3, b)]
+    counts[1030] = 70
+    cached = rng.integers(0, 30, b)
+    lengths = [int(a + c) for a, c in zip(counts, cached)]
+    cache = Cache(ctx, rng, lengths, 7, 16, hkv, d)
+    starts = starts_of(counts)
+    n = int(starts[-1])
+    q, k, v = (rng.standard_normal((n, h, d)).astype(np.float16) for h in (hq, hkv, hkv))
+    hold(paged(ctx, cache, q, starts, hq), *paged_want(cache, q, starts, True), "paged")
+    batch = ctx.begin_batch()
+    out = batch.attention_packed(*[ctx.tensor(x.view(np.uint16)) for x in (q, k, v)], ctx.tensor(starts, U32),
+                                 AttentionConfig(hq, hkv, d))
+    batch.finish()
+    hold(ctx.download(out), *packed_want(q, k, v, starts, True), "packed")
+    q = rng.standard_normal((b, hq, d)).astype(np.float16)
+    hold(decode(ctx, cache, q, hq), *decode_want(cache, q), "decode")
+    x, weights = rows_for(rng, n, hq, hkv, d)
+    check_append(ctx, cache, x, starts, weights)
+
+
+def test_pages_past_four_gib(ctx):
+    """Pools of 9 GB: the first page, the last, and one on either side of 2^32 bytes and of
+    2^32 elements."""
+    rng = np.random.default_rng(64)
+    hq, hkv, d, size = 16, 8, 128, 64
+    page = size * hkv * d
+    pages = 2 ** 32 // page + 4000
+    ids = [0, pages - 1, 2 ** 31 // page - 1, 2 ** 31 // page, 2 ** 32 // page - 1, 2 ** 32 // page]
+    lengths, table = [160, 6 * size - 3], np.array([[1, 3, 5, 0, 0, 0], range(6)])
+    store = [ctx.empty((pages, hkv, size, d)) for _ in "kv"]
+    rows = []
+    for t in store:
+        kv = rng.standard_normal((6, size, hkv, d)).astype(np.float16)
+        for at, one in zip(ids, kv):
+            ctx.upload(t.view((hkv, size, d), (size * d, d, 1), offset=at * page),
+                       np.ascontiguousarray(one.transpose(1, 0, 2)).view(np.uint16))
+        rows.append(kv)
+    views = [t.view((pages, size, hkv, d), (page, d, size * d, 1)) for t in store]
+    held = [tuple(kv[table[i]].reshape(-1, hkv, d)[:n] for kv in rows) for i, n in enumerate(lengths)]
+    dev_table = ctx.tensor(np.array(ids, np.uint32)[table], U32)
+    dev_lengths = ctx.tensor(np.array(lengths, np.uint32), U32)
+    cfg = AttentionConfig(hq, hkv, d)
+    counts = [20, 3]
+    starts = starts_of(counts)
+    q = rng.standard_normal((23, hq, d)).astype(np.float16)
+    new = [rng.standard_normal((2, h, d)).astype(np.float16) for h in (hq, hkv, hkv)]
+    one, many = ctx.tensor(q[:2].view(np.uint16)), ctx.tensor(q.view(np.uint16))
+    batch = ctx.begin_batch()
+    a = batch.attention_decode_paged(one, *views, dev_table, dev_lengths, cfg)
+    c = batch.attention_paged(many, *views, dev_table, dev_lengths, ctx.tensor(starts, U32), cfg)
+    batch.qk_norm_rope_paged(*[ctx.tensor(x.view(np.uint16)) for x in new], None, None, *views, dev_table, dev_lengths,
+                             QkNormRopeCacheConfig(0, THETA, EPS))
+    batch.finish()
+    got_one, got_many = ctx.download(a), ctx.download(c)
+    for i, (k, v) in enumerate(held):
+        n = len(k)
+        hold(got_one[i:i + 1], *attend(q[i:i + 1].astype(np.float64), k, v, [np.arange(n)], False), "decode")
+        s, e = starts[i], starts[i + 1]
+        seen = [np.arange(n - counts[i] + t + 1) for t in range(counts[i])]
+        hold(got_many[s:e], *attend(q[s:e].astype(np.float64), k, v, seen, True), "paged")
+        at, slot = ids[table[i][(n - 1) // size]], (n - 1) % size
+        last = [ctx.download(t.view((hkv, d), (size * d, 1), offset=at * page + slot * d)) for t in store]
+        assert np.array_equal(last[1], new[2][i].view(np.uint16)), "value"
+        hold(last[0], *[x[0] for x in rotated(new[1][i:i + 1], None, np.array([n - 1]))], "key")
