@@ -40,7 +40,7 @@ constexpr int BM = kPrefillBlockM;  // rows per workgroup
 // reference's (a long tail of them counts); it cancels against the row sum.
 constexpr float kBias = 8.0f;
 // Fewest key tiles of a piece of a cut row tile, and most pieces.
-constexpr uint32_t kLeastPiece = 4, kMostPieces = 32;
+constexpr uint32_t kLeastPiece = 8, kMostPieces = 32;
 // More pieces than kOneJoin are joined a few at a time by several workgroups, and then those
 // joins: about the square root of their number. (64 rows of 64 heads on 4000 keys, 16 pieces
 // a tile: 48 us by one workgroup each, 42 us four at a time.)
@@ -514,7 +514,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
       constexpr int AHEAD = 4;
       uint4 kf[AHEAD], vf[AHEAD];
       auto read_k = [&](int c) __attribute__((always_inline)) {
-        kf[c % AHEAD] = *reinterpret_cast<const uint4 *>((ST ? k_lds_a : k_lds_b) + n * D + (((2 * c + h) ^ k_swizzle<D>(n)) * 8));
+        const uint16_t *kp = (ST ? k_lds_a : k_lds_b) + (32 * (c / DC) + n) * D + (((2 * (c % DC) + h) ^ k_swizzle<D>(n)) * 8);
+        kf[c % AHEAD] = *reinterpret_cast<const uint4 *>(kp);
       };
       auto read_v = [&](int i) __attribute__((always_inline)) {
         const uint16_t *v0 = v_lds + 16 * (i / DT) * D + tr_off + ((4 * (i % DT) + tr_chunk) ^ v_swizzle<D>(tr_key)) * 8;
@@ -528,20 +529,25 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
         const float mc = m_run * c2 - kBias;
         float ps0 = 0.0f, ps1 = 0.0f, even = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) nx[0][r] = 0.0f;
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) nx[mt][r] = 0.0f;
 #pragma unroll
         for (int c = 0; c < AHEAD; ++c) read_k(c);
 #pragma unroll
-        for (int c = 0; c < DC; ++c) {
+        for (int c = 0; c < MT * DC; ++c) {
+          // One product, the read of a later one's operand, and one of the tile's 16 MT weights.
+          static_assert(DC == 16 || !PIPE, "a weight per product");
+          const int mt = c / DC, r = c % 16;
           __builtin_amdgcn_sched_barrier(0);
-          nx[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(kf[c % AHEAD]), qop[c], nx[0], 0, 0, 0);
-          if (c + AHEAD < DC) read_k(c + AHEAD);
-          else read_v(c + AHEAD - DC);
-          const float e = exp2_raw(fmaf(s[0][c], c2, -mc));
-          if (c & 1) {
-            pw[0][c >> 1] = pack_f16x2(even, e);
-            if (c & 2) ps1 = dot2(pw[0][c >> 1], 0x3c003c00u, ps1);
-            else ps0 = dot2(pw[0][c >> 1], 0x3c003c00u, ps0);
+          nx[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(kf[c % AHEAD]), qop[c % DC], nx[mt], 0, 0, 0);
+          if (c + AHEAD < MT * DC) read_k(c + AHEAD);
+          else read_v(c + AHEAD - MT * DC);
+          const float e = exp2_raw(fmaf(s[mt][r], c2, -mc));
+          if (r & 1) {
+            pw[mt][r >> 1] = pack_f16x2(even, e);
+            if (r & 2) ps1 = dot2(pw[mt][r >> 1], 0x3c003c00u, ps1);
+            else ps0 = dot2(pw[mt][r >> 1], 0x3c003c00u, ps0);
           }
           even = e;
         }
@@ -572,12 +578,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
       // O^T[d][row] += V^T[d][keys] P^T[keys][row], 16-key chunks.
       if constexpr (PIPE) {
 #pragma unroll
-        for (int i = 0; i < 2 * DT; ++i) {
-          const int base = i / DT * 4;
-          const h8_t pb = as_h8(make_uint4(pw[0][base], pw[0][base + 1], pw[0][base + 2], pw[0][base + 3]));
+        for (int i = 0; i < BN / 16 * DT; ++i) {
+          const int mt = i / DT >> 1, base = (i / DT & 1) * 4;
+          const h8_t pb = as_h8(make_uint4(pw[mt][base], pw[mt][base + 1], pw[mt][base + 2], pw[mt][base + 3]));
           __builtin_amdgcn_sched_barrier(0);
           o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(vf[i % AHEAD]), pb, o[i % DT], 0, 0, 0);
-          if (i + AHEAD < 2 * DT) read_v(i + AHEAD);
+          if (i + AHEAD < BN / 16 * DT) read_v(i + AHEAD);
         }
         __builtin_amdgcn_sched_barrier(0);
       } else {
