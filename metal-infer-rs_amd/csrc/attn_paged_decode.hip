@@ -1,12 +1,12 @@
 // Attention of one new token per sequence over its pages (head_dim 32, 64, 128, 256).
 //
 // Bound by the bytes of K and V, each read once per chunk of up to 16 query heads.
-//  - Split: a unit is (sequence, KV head, chunk). With many units, every wave takes an
-//    equal share of the (unit, 32-key tile) space of all sequences, as the lengths on the
-//    device say, and goes through it by itself with an online softmax: no barriers, and
-//    while one wave ends a part the others keep loading. With few units, which would be in
-//    too many parts, each workgroup takes one piece of a unit and its waves, on
-//    interleaved tiles, merge through LDS.
+//  - Split: a unit is (sequence, KV head, chunk). Where pieces of one length divide all
+//    units about evenly over the workgroups, each workgroup takes one piece and its waves,
+//    on interleaved tiles, merge through LDS. Else every wave takes an equal share of the
+//    (unit, 32-key tile) space of all sequences, as the lengths on the device say, and goes
+//    through it by itself with an online softmax: no barriers, and while one wave ends a
+//    part the others keep loading.
 //  - A part that is not its whole unit leaves its max, sum and weighted values (f32), and
 //    the last of a unit's parts to finish joins them in order, so the result does not
 //    depend on which one that is.
@@ -38,9 +38,9 @@ typedef float f4_t __attribute__((ext_vector_type(4)));
 constexpr uint32_t per_cu(uint32_t) { return 2; }
 // Fewest tiles of a workgroup's piece (one per wave) and of a wave's share.
 constexpr uint32_t kPiece = kWaves, kShare = 2;
-// Units from which each wave works by itself; more than twice kJoin pieces are joined in
-// steps of kJoin.
-constexpr uint32_t kManyUnits = 128, kJoin = 16;
+// Pieces may be longer than an even share by this many eighths; more than twice kJoin of a
+// unit's are joined in steps of kJoin.
+constexpr uint32_t kUneven = 2, kJoin = 16;
 
 __device__ __forceinline__ float lane_value(float x, int lane) {
   return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), lane));
@@ -84,17 +84,23 @@ __device__ __forceinline__ Share share_work(const PagedDecodeParams &p, uint32_t
   Share sh{0, 0, tiles * upb};
   if (few * upb <= W || !__any(longer)) {
     sh.piece = kPiece, sh.total = few * upb;
-  } else if (used * upb < kManyUnits) {
-    // The smallest pieces that give each workgroup one at most, within an eighth.
-    sh.piece = (tiles * upb + W - 1) / W;
-    for (;;) {
+  } else {
+    // The smallest pieces that give each workgroup one at most, if they are near an even
+    // share: a workgroup's four waves on one piece need no joins but that piece's, but the
+    // longest piece sets the time. 32 equal sequences of 4096 keys (8 KV heads of 128) take 89
+    // us so and 93 by shares of waves; 32 of 500 to 8000 keys 116 and 103.
+    const uint32_t even = (tiles * upb + W - 1) / W, most = used * upb > W ? 0 : even + even * kUneven / 8;
+    for (uint32_t piece = even; piece <= most; piece += (piece + 7) / 8) {
       uint32_t pieces = 0;
       for (uint32_t c0 = 0; c0 < p.batch; c0 += 64)
-        if (c0 + lane < p.batch) pieces += (s_tiles[c0 + lane] + sh.piece - 1) / sh.piece;
+        if (c0 + lane < p.batch) pieces += (s_tiles[c0 + lane] + piece - 1) / piece;
       sh.total = last_lane(scan64(pieces)) * upb;
-      if (sh.total <= W || sh.piece >= tiles) break;
-      sh.piece += (sh.piece + 7) / 8;
+      if (sh.total <= W) {
+        sh.piece = piece;
+        break;
+      }
     }
+    if (sh.piece == 0) sh.total = tiles * upb;
   }
   const uint32_t takers = sh.piece != 0 ? W : W * kWaves;
   sh.seg = max((sh.total + takers - 1) / takers, sh.piece != 0 ? 1u : kShare);
