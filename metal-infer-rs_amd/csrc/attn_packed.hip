@@ -13,14 +13,21 @@
 //    (ds_read_b64_tr_b16);
 //  - the next tile's direct global -> LDS loads are in flight while one is computed. A
 //    wave loads 16 (or 8) consecutive rows of a tile, so they lie in one page.
+//  - at head_dim 256 a wave's accumulators and Q leave room for one wave per SIMD, so the
+//    next tile's scores are computed beside this one's softmax, each operand read four
+//    products ahead, in the source's order (three prompts of 1000 to 3000 rows, 16 heads on
+//    4: 158 us, and 180 us where the products wait for the softmax and for LDS).
 //  - Order: the work per row tile is known on the device only. Every workgroup works out
 //    the same plan from the sequences' rows and lengths and takes the piece of its rank:
 //    tiles with more keys than a workgroup's even share are cut into pieces, which come
 //    first, then the whole tiles with most keys first. The pieces of a cut tile leave
 //    their max, sum and weighted values (f32), and the last of them to finish joins them
 //    in order.
-// Bound by the matrix instructions with the exponentials beside them for long prompts,
-// by the bytes of K and V for a few rows on a long cache.
+// Bound by the matrix instructions with the exponentials beside them for long prompts (two
+// of 4000 to 6000 rows, 32 heads on 8 of 128: 415 us, 1.0 PFLOP/s, a large f16 product's rate
+// being 1.34), by the bytes of K and V for a few rows on a long cache, and for short prompts
+// by what every row tile needs once: its place in the plan (2.5 us), Q and the first tile
+// (3 us) and the output (1.5 us), beside two such workgroups per CU.
 #include <type_traits>
 
 #include "paged_tile.hpp"
@@ -33,13 +40,17 @@ namespace {
 using namespace mi::dev;
 
 // Keys per tile: at head_dim 256 half as many, as the accumulators and Q take half of a
-// wave's registers.
+// wave's registers (64 keys there spill: 233 us instead of 152 for three prompts of 1000 to
+// 3000 rows).
 constexpr int tile_keys(int head_dim) { return head_dim == 256 ? 32 : kPrefillBlockN; }
 constexpr int BM = kPrefillBlockM;  // rows per workgroup
 // Added to every weight's exponent, so that f16 holds weights down to 2^-32 of the
 // reference's (a long tail of them counts); it cancels against the row sum.
 constexpr float kBias = 8.0f;
-// Fewest key tiles of a piece of a cut row tile, and most pieces.
+// Fewest key tiles of a piece of a cut row tile, and most pieces: a join costs as much as
+// some tiles (64 rows of 64 heads on 4000 keys: 32 us with at least 8, 42 us with 4), and the
+// time of many pieces' joins grows with them (32 rows of 32 heads on 16384 keys: 41, 38 and
+// 49 us with up to 16, 32 and 64; 272 us uncut).
 constexpr uint32_t kLeastPiece = 8, kMostPieces = 32;
 // More pieces than kOneJoin are joined a few at a time by several workgroups, and then those
 // joins: about the square root of their number. (64 rows of 64 heads on 4000 keys, 16 pieces
@@ -175,7 +186,8 @@ __device__ __forceinline__ bool plan_piece(const PackedParams &p, uint32_t rank,
   }
   if (found) return true;
   // The whole tiles, most key tiles first: the largest x of which more than rank tiles
-  // have at least x.
+  // have at least x. (Seven prompts of 150 to 1500 rows, 40 heads on 8: 95 us, 103 us in the
+  // order of the rows; forty of 100 to 500 at head_dim 64 53 and 50 us.)
   rank -= pieces;
   if (rank >= all - cuts) return false;
   auto at_least = [&](uint32_t x) -> uint32_t {
@@ -231,7 +243,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   constexpr int BPW = RPW / RPB;       // its direct loads of K (and V) per tile
   constexpr uint32_t GROUPS = BN / 16, HELD = 64 / GROUPS;  // 16-key groups per tile; tiles whose page ids a wave holds
   constexpr int DC = D / 16, DT = D / 32;
-  constexpr bool PIPE = D == 256;
+  constexpr bool PIPE = D == 256;      // one wave per SIMD
   constexpr int TILE = BN * D, OUT = 64 * D;  // halves of a tile, and of two waves' output rows
   // One array per stage, and the stage a compile-time choice, so that the compiler can
   // tell the loads into one from the reads of the other.
