@@ -411,9 +411,9 @@ mi_status mi_decode_step_attention(mi_batch *batch, const mi_tensor *q,
  *    they are in every output.
  *  - Paged cache: key_pages / value_pages [P, S, Hkv, D], any strides with unit
  *    innermost stride (storage [P, Hkv, S, D] keeps a head's keys together), S a
- *    power of two of at least 16. block_table, device u32 [B, M] (any row
- *    stride): position p of sequence b is in page block_table[b, p / S] at
- *    p % S. An id of P or more names no page: no row sees its keys, and a row
+ *    power of two from 16 to 2^20. block_table, device u32 [B, M] (any row
+ *    stride, M * S below 2^31): position p of sequence b is in page
+ *    block_table[b, p / S] at p % S. An id of P or more names no page: no row sees its keys, and a row
  *    that would be stored there is not. Sequences may share pages that they only
  *    read; which of two rows written to one slot stays is not defined.
  *  - lengths, device u32 [B]: keys of each sequence with the step's rows
@@ -424,8 +424,8 @@ mi_status mi_decode_step_attention(mi_batch *batch, const mi_tensor *q,
  *    result, whatever they hold.
  *  - head_dim 32, 64, 128 or 256, any group of query heads; bases and outer
  *    strides of f16 tensors multiples of 16 bytes, position strides of keys and
- *    values not negative. config->query_offset (and the transform's offset) are
- *    ignored. Nothing is launched for N = 0 or B = 0.
+ *    values not negative, a page (or 64 packed rows) of them within 2 GiB.
+ *    config->query_offset (and the transform's offset) are ignored. Nothing is launched for N = 0 or B = 0.
  *  - Tables, lengths and row offsets are read when the call runs on the GPU: a
  *    captured call reads what they hold at each replay. Outputs must not overlap
  *    inputs, except the transform's q_out, which may be q itself. */

@@ -1,5 +1,6 @@
 // What the kernels over packed rows and the paged KV cache share: which sequence a
-// row belongs to, and where the rows that no sequence has are read from.
+// row belongs to, where the rows that no sequence has are read from, scans over a wave,
+// direct loads into LDS and the waits for them.
 #pragma once
 
 #include "device_common.hpp"
@@ -8,7 +9,7 @@
 namespace mi {
 namespace dev {
 
-// A key row of zeros (the largest head_dim). Rows of a tile past its last key, and
+// A key row of zeros (the largest head_dim). Rows of a decode tile past its last key, and
 // those of a page that is not there, are read from here: a masked weight is 0, and 0
 // times what a recycled page holds (infinities, NaN) would be NaN in the products.
 static __device__ __attribute__((aligned(512))) uint16_t zero_row[256];
