@@ -852,3 +852,100 @@ def test_pages_past_four_gib(ctx):
         last = [ctx.download(t.view((hkv, d), (size * d, 1), offset=at * page + slot * d)) for t in store]
         assert np.array_equal(last[1], new[2][i].view(np.uint16)), "value"
         hold(last[0], *[x[0] for x in rotated(new[1][i:i + 1], None, np.array([n - 1]))], "key")
+
+
+# ------------------------------------------------------------ layouts, sharing --
+
+def spread_out(ctx, n, h, d):
+    """An output in head-major storage with a gap between rows: (owner, view of [n, h, d])."""
+    owner = ctx.tensor(np.full((h, n, d + 8), 0x1234, np.uint16))
+    return owner, owner.view((n, h, d), (d + 8, n * (d + 8), 1))
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(6, 2, 128), (5, 5, 64), (4, 1, 256), (8, 4, 32)])
+def test_outputs_and_queries_in_other_layouts(ctx, hq, hkv, d):
+    """Head-major queries and outputs with gaps, of which nothing but the rows is written; keys
+    and values of one head that all KV heads share (a head stride of 0)."""
+    rng = np.random.default_rng(71)
+    counts, cached = [3, 1, 40], [20, 700, 0]
+    starts = starts_of(counts)
+    n = int(starts[-1])
+    cache = Cache(ctx, rng, [a + b for a, b in zip(counts, cached)], 50, 16, hkv, d, "gaps")
+    q = rng.standard_normal((n, hq, d)).astype(np.float16)
+    store = np.full((hq, n, d + 16), 0x7E00, np.uint16)
+    store[:, :, :d] = q.view(np.uint16).transpose(1, 0, 2)
+    owner = ctx.tensor(store)
+    view = owner.view((n, hq, d), (d + 16, n * (d + 16), 1))
+    pages = (cache.key_pages, cache.value_pages, cache.device_table, cache.device_lengths)
+    k, v = (rng.standard_normal((n, 1, d)).astype(np.float16) for _ in "kv")
+    shared = [ctx.tensor(x.view(np.uint16)) for x in (k, v)]
+    outs = [spread_out(ctx, n, hq, d), spread_out(ctx, n, hq, d), spread_out(ctx, 3, hq, d)]
+    cfg, dev_starts = AttentionConfig(hq, hkv, d), ctx.tensor(starts, U32)
+    batch = ctx.begin_batch()
+    batch.attention_paged(view, *pages, dev_starts, cfg, out=outs[0][1])
+    batch.attention_packed(view, *[t.view((n, hkv, d), (d, 0, 1)) for t in shared], dev_starts, cfg, out=outs[1][1])
+    batch.attention_decode_paged(owner.view((3, hq, d), (d + 16, n * (d + 16), 1)), *pages, cfg, out=outs[2][1])
+    batch.finish()
+    wants = (paged_want(cache, q, starts, True),
+             packed_want(q, np.repeat(k, hkv, 1), np.repeat(v, hkv, 1), starts, True), decode_want(cache, q[:3]))
+    for (store, _), (want, tol) in zip(outs, wants):
+        raw = ctx.download(store)
+        assert (raw[:, :, d:] == 0x1234).all(), "the gap between rows was written"
+        hold(raw[:, :, :d].transpose(1, 0, 2), want, tol)
+
+
+def test_sequences_that_share_pages(ctx):
+    """A prompt's pages in three tables, each with a page of its own behind them."""
+    rng = np.random.default_rng(72)
+    hq, hkv, d, size = 8, 2, 128, 16
+    cache = Cache(ctx, rng, [100, 100, 100], 7, size, hkv, d)
+    cache.table[1:, :6] = cache.table[0, :6]
+    cache.device_table = cache.upload_table()
+    for i in (1, 2):
+        cache.rows[i] = tuple(np.concatenate([a[:96], b[96:]]) for a, b in zip(cache.rows[0], cache.rows[i]))
+    q = rng.standard_normal((3, hq, d)).astype(np.float16)
+    hold(decode(ctx, cache, q, hq), *decode_want(cache, q))
+    starts = starts_of([4, 4, 4])
+    q = rng.standard_normal((12, hq, d)).astype(np.float16)
+    hold(paged(ctx, cache, q, starts, hq), *paged_want(cache, q, starts, True))
+
+
+def test_two_contexts_at_once(ctx):
+    """Calls of two contexts in flight together, each with pieces to join, match single ones."""
+    rng = np.random.default_rng(73)
+    hq, hkv, d = 8, 2, 128
+    other = mi_attn.Context(0)
+    try:
+        sides = []
+        for c in (ctx, other):
+            cache = Cache(c, rng, [3000, 900, 40], 190, 16, hkv, d)
+            starts = starts_of([1, 60, 3])
+            q = rng.standard_normal((64, hq, d)).astype(np.float16)
+            sides.append((c, cache, c.tensor(q.view(np.uint16)), c.tensor(starts, U32), q, starts))
+        cfg = AttentionConfig(hq, hkv, d)
+
+        def enqueue(side):
+            c, cache, t, dev_starts, _, _ = side
+            pages = (cache.key_pages, cache.value_pages, cache.device_table, cache.device_lengths)
+            batch = c.begin_batch()
+            out = [c.empty((64, hq, d)), c.empty((3, hq, d))]
+            for _ in range(5):
+                batch.attention_paged(t, *pages, dev_starts, cfg, out=out[0])
+                batch.attention_decode_paged(t.view((3, hq, d), (hq * d, d, 1)), *pages, cfg, out=out[1])
+            return batch, out
+
+        alone = []
+        for side in sides:
+            batch, out = enqueue(side)
+            batch.finish()
+            alone.append([side[0].download(o) for o in out])
+            hold(alone[-1][0], *paged_want(side[1], side[4], side[5], True))
+        both = [enqueue(side) for side in sides]
+        for batch, _ in both:
+            batch.finish()
+        for side, (_, out), want in zip(sides, both, alone):
+            for o, w in zip(out, want):
+                assert np.array_equal(side[0].download(o), w)
+        del both, sides, out, o
+    finally:
+        other.close()
