@@ -95,17 +95,6 @@ struct Tiles {
   }
 };
 
-// Sum and largest value over the 64 lanes, to every lane.
-__device__ __forceinline__ uint32_t wave_sum(uint32_t x) { return last_lane(scan64(x)); }
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
-  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false));
-}
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-  x = dpp_max<0x118, 0xf>(dpp_max<0x114, 0xf>(dpp_max<0x112, 0xf>(dpp_max<0x111, 0xf>(x))));
-  return last_lane(dpp_max<0x143, 0xc>(dpp_max<0x142, 0xa>(x)));
-}
-
 // What the workgroup of a rank does: key tiles [begin, end) of a row tile, as piece
 // `piece` of `pieces`; `cut` numbers the tiles that are cut.
 struct Piece {

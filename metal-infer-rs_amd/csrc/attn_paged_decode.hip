@@ -3,10 +3,10 @@
 // Bound by the bytes of K and V, each read once per chunk of up to 16 query heads.
 //  - Split: a unit is (sequence, KV head, chunk). Where pieces of one length divide all
 //    units about evenly over the workgroups, each workgroup takes one piece and its waves,
-//    on interleaved tiles, merge through LDS. Else every wave takes an equal share of the
-//    (unit, 32-key tile) space of all sequences, as the lengths on the device say, and goes
-//    through it by itself with an online softmax: no barriers, and while one wave ends a
-//    part the others keep loading.
+//    on interleaved tiles, merge through LDS. Many units of about equal length are a wave's
+//    each. Else every wave takes an equal share of the (unit, 32-key tile) space of all
+//    sequences, as the lengths on the device say, and goes through it by itself with an
+//    online softmax: no barriers, and while one wave ends a part the others keep loading.
 //  - A part that is not its whole unit leaves its max, sum and weighted values (f32), and
 //    the last of a unit's parts to finish joins them in order, so the result does not
 //    depend on which one that is.
@@ -41,6 +41,7 @@ constexpr uint32_t kPiece = kWaves, kShare = 2;
 // Pieces may be longer than an even share by this many eighths; more than twice kJoin of a
 // unit's are joined in steps of kJoin.
 constexpr uint32_t kUneven = 2, kJoin = 16;
+constexpr uint32_t kJoinTiles = 12;  // tiles that take as long as shares' partials and joins
 
 __device__ __forceinline__ float lane_value(float x, int lane) {
   return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), lane));
@@ -59,17 +60,17 @@ __device__ __forceinline__ float sum32(float x) {
 }
 
 // How a launch divides its work, the same in every wave. With `piece` a position is a
-// piece of that many tiles of a unit, for a workgroup, else a tile, for a wave; each
-// takes `seg` of them. s_tiles[b] gets the sequences' tiles, s_pre[b] the positions of
+// piece of that many tiles of a unit, for a workgroup, else a tile, or with `whole` a unit,
+// for a wave; each takes `seg` of them. s_tiles[b] gets the sequences' tiles, s_pre[b] the positions of
 // all units before b's. Every wave computes all of it and reads back what it wrote
 // itself, so no barrier is needed (the waves write the same values).
 struct Share {
   uint32_t piece, seg, total;
+  bool whole;
 };
 __device__ __forceinline__ Share share_work(const PagedDecodeParams &p, uint32_t upb, uint32_t *s_tiles,
                                             uint32_t *s_pre, int lane) {
-  uint32_t tiles = 0, few = 0, used = 0;  // tiles, pieces of kPiece, sequences with a key
-  bool longer = false;                    // than one piece
+  uint32_t tiles = 0, few = 0, used = 0, longest = 0;  // tiles, pieces of kPiece, sequences with a key
   for (uint32_t c0 = 0; c0 < p.batch; c0 += 64) {
     const uint32_t b = c0 + lane;
     const uint32_t t = b < p.batch ? (paged_length(p.kv, b) + kDecodeTile - 1) / kDecodeTile : 0;
@@ -77,13 +78,21 @@ __device__ __forceinline__ Share share_work(const PagedDecodeParams &p, uint32_t
     tiles += t;
     few += (t + kPiece - 1) / kPiece;
     used += (uint32_t)__popcll(__ballot(t != 0));
-    longer |= t > kPiece;
+    longest = max(longest, t);
   }
-  tiles = last_lane(scan64(tiles)), few = last_lane(scan64(few));
+  tiles = wave_sum(tiles), few = wave_sum(few), longest = wave_max(longest);
   const uint32_t W = gridDim.x;
-  Share sh{0, 0, tiles * upb};
-  if (few * upb <= W || !__any(longer)) {
+  Share sh{0, 0, tiles * upb, false};
+  if (few * upb <= W) {
     sh.piece = kPiece, sh.total = few * upb;
+  } else if (const uint32_t units = used * upb, waves = W * kWaves;
+             longest <= kPiece ||
+             (2 * units >= waves && (units + waves - 1) / waves * longest <= tiles * upb / waves + kJoinTiles)) {
+    // More units than workgroups, of a piece at most: a wave each (808 of one tile, D = 128:
+    // 7.5 us, by workgroups 11.7). The same where that keeps half of the waves busy and the
+    // longest is not far from an even share (1024 of 400 to 511 keys: 48 us, in shares 60;
+    // 512 of 300 to 400 at D = 256 59 and 42).
+    sh.whole = true, sh.total = units;
   } else {
     // The smallest pieces that give each workgroup one at most, if they are near an even
     // share: a workgroup's four waves on one piece need no joins but that piece's, but the
@@ -103,11 +112,12 @@ __device__ __forceinline__ Share share_work(const PagedDecodeParams &p, uint32_t
     if (sh.piece == 0) sh.total = tiles * upb;
   }
   const uint32_t takers = sh.piece != 0 ? W : W * kWaves;
-  sh.seg = max((sh.total + takers - 1) / takers, sh.piece != 0 ? 1u : kShare);
+  sh.seg = max((sh.total + takers - 1) / takers, sh.piece != 0 || sh.whole ? 1u : kShare);
   uint32_t carry = 0;
   for (uint32_t c0 = 0; c0 < p.batch; c0 += 64) {
     const uint32_t b = c0 + lane;
     uint32_t x = b < p.batch ? s_tiles[b] : 0;
+    if (sh.whole) x = min(x, 1u);
     if (sh.piece != 0) x = (x + sh.piece - 1) / sh.piece;
     x = scan64(x * upb);
     if (b < p.batch) s_pre[b + 1] = carry + x;
@@ -293,6 +303,8 @@ __global__ __launch_bounds__(kWaves * 64, per_cu(D)) void attn_decode_paged_kern
       t0 = piece * sh.piece;
       t1 = min(tiles, t0 + sh.piece);
       slot = pos;
+    } else if (sh.whole) {
+      j = rel, t0 = 0, t1 = tiles, piece = 0, pieces = 1, slot = 0;
     } else {
       j = rel / tiles;
       t0 = rel - j * tiles;
@@ -505,7 +517,7 @@ __global__ __launch_bounds__(kWaves * 64, per_cu(D)) void attn_decode_paged_kern
       }
       __syncthreads();  // the next piece's loads overwrite the stages
     }
-    pos += together ? 1 : t1 - t0;
+    pos += together || sh.whole ? 1 : t1 - t0;
     if (pos < end && pos >= s_pre[b + 1]) b = sequence_at(pos);
   }
   // The joins come after the loop, so that they take none of its registers: what they

@@ -949,3 +949,16 @@ def test_two_contexts_at_once(ctx):
         del both, sides, out, o
     finally:
         other.close()
+
+
+@pytest.mark.parametrize("hq,hkv,d,size,batch,low,high", [
+    (16, 16, 64, 16, 70, 0, 128), (64, 32, 32, 16, 70, 100, 260), (16, 8, 128, 16, 300, 0, 33), (16, 16, 256, 16, 40, 1, 60)])
+def test_decode_of_many_short_units(ctx, hq, hkv, d, size, batch, low, high):
+    """More units than workgroups, each a wave's own; several in turn; some without a key."""
+    rng = np.random.default_rng(65)
+    lengths = [int(n) for n in rng.integers(low, high, batch)]
+    cache = Cache(ctx, rng, lengths, -(-high // size), size, hkv, d, missing=[(1, 0), (batch - 1, 0)])
+    q = (1.5 * rng.standard_normal((batch, hq, d))).astype(np.float16)
+    got = decode(ctx, cache, q, hq)
+    hold(got, *decode_want(cache, q), f"decode {batch} x {hkv}")
+    assert np.array_equal(got, decode(ctx, cache, q, hq)), "two calls differ"
