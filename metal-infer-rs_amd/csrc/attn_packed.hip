@@ -71,26 +71,27 @@ struct Rows {
 // to tile, else all are the same.
 template <int BN>
 struct Tiles {
-  uint32_t group, causal;
+  Divisor group;
+  uint32_t causal;
   // Keys that the last row of tile i sees, of `tokens` tokens.
   __device__ __forceinline__ uint32_t of(int32_t first, uint32_t tokens, uint32_t i) const {
-    const uint32_t last = causal != 0 ? min(tokens - 1, ((i + 1) * BM - 1) / group) : tokens - 1;
+    const uint32_t last = causal != 0 ? min(tokens - 1, divide((i + 1) * BM - 1, group)) : tokens - 1;
     return ((uint32_t)max(0, first + (int32_t)last + 1) + BN - 1) / BN;
   }
   __device__ __forceinline__ Rows sequence(int32_t first, uint32_t tokens) const {
-    const uint32_t n = (tokens * group + BM - 1) / BM;
+    const uint32_t n = (tokens * group.value + BM - 1) / BM;
     return n == 0 ? Rows{0, 0, 0, 0} : Rows{n, of(first, tokens, 0), of(first, tokens, n - 1), first};
   }
   // The first row tile with at least x key tiles (the count of them if none has): that of
   // the first token that sees key (x - 1) BN.
   __device__ __forceinline__ uint32_t first_with(Rows r, uint32_t x) const {
-    const uint32_t i = (uint32_t)((int32_t)((x - 1) * BN) - r.first) * group / BM;
+    const uint32_t i = (uint32_t)((int32_t)((x - 1) * BN) - r.first) * group.value / BM;
     return x <= r.least ? 0 : x > r.most ? r.tiles : i;
   }
   // Key tiles of tile i.
   __device__ __forceinline__ uint32_t at(Rows r, uint32_t i) const {
     if (causal == 0 || i + 1 >= r.tiles) return r.most;
-    const int32_t last = (int32_t)(((i + 1) * BM - 1) / group);
+    const int32_t last = (int32_t)divide((i + 1) * BM - 1, group);
     return ((uint32_t)max(0, r.first + last + 1) + BN - 1) / BN;
   }
 };
@@ -247,21 +248,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 31, h = lane >> 5;
-  const uint32_t G = p.group;
+  const uint32_t G = p.group.value;
 
   // Workgroups go round-robin over the 8 XCDs: where the KV heads divide evenly, each
   // XCD takes whole heads, whose K and V stay in its L2.
   uint32_t kvh, rest;
   {
-    const uint32_t id = blockIdx.x, H = p.kv_heads;
-    if (H % 8 == 0) {
-      const uint32_t xcd = id % 8, k = id / 8, per = H / 8;
-      kvh = xcd * per + k % per;
-      rest = k / per;
-    } else {
-      kvh = id % H;
-      rest = id / H;
-    }
+    const bool whole = p.kv_heads % 8 == 0;
+    const uint32_t per = p.heads_apart.value, k = whole ? blockIdx.x / 8 : blockIdx.x;
+    rest = divide(k, p.heads_apart);
+    kvh = k - rest * per + (whole ? blockIdx.x % 8 * per : 0);
   }
   // The sequences' rows and first positions (every wave writes all of them, and reads back
   // what it wrote itself), and the piece of this rank.
@@ -270,7 +266,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     if (bb >= p.batch) continue;
     const RowRange r = sequence_rows(p.row_starts, bb, p.rows);
     const uint32_t tokens = r.end - r.begin;
-    s_rows[bb] = Tiles<BN>{G, p.causal}.sequence(PAGED ? (int32_t)paged_length(p.kv, bb) - (int32_t)tokens : 0, tokens);
+    s_rows[bb] = Tiles<BN>{p.group, p.causal}.sequence(PAGED ? (int32_t)paged_length(p.kv, bb) - (int32_t)tokens : 0, tokens);
   }
   Piece pc;
   if (!plan_piece<BN>(p, rest, s_rows, s_before, lane, &pc)) return;
@@ -282,9 +278,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   const int64_t off = (int64_t)L - tokens;  // position of the first row (negative: more rows than keys)
 
   const uint32_t row0 = tile * BM, my_row = row0 + wave * 32 + n;
-  const uint32_t my_t = my_row / G, my_g = my_row % G;
+  const uint32_t my_t = divide(my_row, p.group), my_g = my_row - my_t * G;
   const bool row_ok = my_t < tokens;
-  const uint32_t t_first = row0 / G, t_last = min(tokens - 1, (row0 + BM - 1) / G);
+  const uint32_t t_first = divide(row0, p.group), t_last = min(tokens - 1, divide(row0 + BM - 1, p.group));
   const uint32_t kmax = p.causal != 0 ? (uint32_t)max((int64_t)0, off + t_last + 1) : L;  // at most L
   const bool active = row0 + wave * 32 < tokens * G;  // whether this wave has rows
   // Last key that this lane's row sees, and that the tile's first row does.
@@ -831,7 +827,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   for (int i = 0; i < 32 / RPI; ++i) {
     const int r = i * RPI + lane_o / CPR;
     const uint4 v = *reinterpret_cast<const uint4 *>(own_rows + r * D + (c_out ^ out_swizzle<D>(r)) * 8);
-    const uint32_t prow = row0 + wave * 32 + r, t = prow / G, g = prow % G;
+    const uint32_t prow = row0 + wave * 32 + r, t = divide(prow, p.group), g = prow - t * G;
     if (t < tokens)
       *reinterpret_cast<uint4 *>(p.out + (int64_t)(range.begin + t) * p.o_tok + (int64_t)(kvh * G + g) * p.o_head +
                                  c_out * 8) = v;

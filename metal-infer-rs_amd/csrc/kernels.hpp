@@ -394,6 +394,18 @@ hipError_t launch_paged_decode(const PagedDecodeParams &p, uint32_t head_dim, co
 
 // Packed query rows [N, Hq, D] of `batch` sequences over their own packed rows of K and
 // V (kv.table null: kv.k_pos and v_pos are row strides), or over their pages.
+// Division of numbers below 2^31 by a known one, in two multiplications instead of some 25
+// instructions: with 2^l >= d, magic = floor(2^(31 + l) / d) + 1 exceeds the quotient by less
+// than 2^l / d, so x magic / 2^(31 + l) exceeds x / d by less than 2^-l <= 1 / d.
+struct Divisor {
+  uint32_t magic, shift, value;
+};
+inline Divisor divisor(uint32_t d) {
+  uint32_t l = 0;
+  while ((1ull << l) < d) ++l;
+  return {(uint32_t)((1ull << (31 + l)) / d + 1), 31 + l, d};
+}
+
 struct PackedParams {
   const uint16_t *q;
   int64_t q_tok, q_head;
@@ -401,7 +413,9 @@ struct PackedParams {
   int64_t o_tok, o_head;
   PagedKv kv;
   const uint32_t *row_starts;
-  uint32_t rows, batch, q_heads, kv_heads, group, causal;
+  uint32_t rows, batch, q_heads, kv_heads, causal;
+  Divisor group;        // query heads of a KV head
+  Divisor heads_apart;  // kv_heads, or an eighth of them where that is whole
   uint32_t row_tiles;  // most row tiles of a KV head (host bound)
   float scale_log2;
   // Row tiles with more than an even share of the keys are cut into pieces: at most

@@ -213,13 +213,15 @@ mi_status packed(mi_batch *batch, const mi_tensor *q, const mi_tensor *key, cons
   p.out = static_cast<uint16_t *>(out->data), p.o_tok = out->stride[0], p.o_head = out->stride[1];
   p.row_starts = static_cast<const uint32_t *>(row_starts->data);
   p.rows = (uint32_t)q->shape[0], p.batch = (uint32_t)sequences;
-  p.q_heads = config->query_heads, p.kv_heads = config->kv_heads, p.group = p.q_heads / p.kv_heads;
+  p.q_heads = config->query_heads, p.kv_heads = config->kv_heads;
+  p.group = kernels::divisor(p.q_heads / p.kv_heads);
+  p.heads_apart = kernels::divisor(p.kv_heads % 8 == 0 ? p.kv_heads / 8 : p.kv_heads);
   p.causal = config->causal != 0 ? 1 : 0;
   p.scale_log2 = scale_log2(config->head_dim);
   // Sequences beyond one launch's go in launches of their own, each with room for all rows.
   const uint32_t step = std::min(p.batch, kernels::kPackedMaxBatch);
-  const uint64_t tiles = kernels::packed_row_tiles(p.rows, step, p.group);
-  if ((uint64_t)p.rows * p.group >= kRows31 || tiles * p.kv_heads + kernels::kSplitCounters >= kRows31)
+  const uint64_t tiles = kernels::packed_row_tiles(p.rows, step, p.group.value);
+  if ((uint64_t)p.rows * p.group.value + kernels::kPrefillBlockM >= kRows31 || tiles * p.kv_heads + kernels::kSplitCounters >= kRows31)
     return fail(MI_ERR_SHAPE, "attention grid exceeds the launch limits");
   if ((st = check_batch(batch)) != MI_OK || q->shape[0] == 0 || sequences == 0) return st;
   p.row_tiles = (uint32_t)tiles;

@@ -75,6 +75,10 @@ __device__ __forceinline__ const Params __attribute__((address_space(4))) *param
   return at;
 }
 
+__device__ __forceinline__ uint32_t divide(uint32_t x, kernels::Divisor d) {
+  return (uint32_t)(((uint64_t)x * d.magic) >> d.shift);
+}
+
 // s_waitcnt vmcnt(N), the other counters left at their maxima.
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
