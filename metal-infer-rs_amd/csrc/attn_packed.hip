@@ -426,7 +426,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     }
   };
 
-  float16_t s_cur[MT];
+  float16_t s_cur[MT];  // with PIPE: the scores of the tile that the next step takes
+  // S^T[key][row] = K Q^T of a tile.
   auto scores = [&](const uint16_t *k_lds, float16_t (&s)[MT]) __attribute__((always_inline)) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -455,10 +456,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
       if constexpr (PIPE) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) s[mt] = s_cur[mt];
+        // The accumulators stay in one half of the register file: left to itself the compiler
+        // moves all of them to the other one and back in every second step.
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) asm volatile("" : "+a"(o[dt]));
       } else {
-        // S^T[key][row]: two 32-key halves, at raised wave priority.
+        // Two 32-key halves, at raised wave priority.
         __builtin_amdgcn_s_setprio(1);
         scores(k_lds, s);
         __builtin_amdgcn_sched_group_barrier(kSchedDsRead, kReadAhead, 0);
@@ -506,22 +509,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
           }
         psum = ps0 + ps1;
       };
-      // The reference moves only when a weight leaves f16's range: the sum is then +inf
-      // or NaN, as it is for a row without a reference yet (m_run = -inf).
-      constexpr int AHEAD = 4;
-      uint4 kf[AHEAD], vf[AHEAD];
+      uint4 kf[kReadAhead], vf[kReadAhead];
       auto read_k = [&](int c) __attribute__((always_inline)) {
         const uint16_t *kp = (ST ? k_lds_a : k_lds_b) + (32 * (c / DC) + n) * D + (((2 * (c % DC) + h) ^ k_swizzle<D>(n)) * 8);
-        kf[c % AHEAD] = *reinterpret_cast<const uint4 *>(kp);
+        kf[c % kReadAhead] = *reinterpret_cast<const uint4 *>(kp);
       };
       auto read_v = [&](int i) __attribute__((always_inline)) {
         const uint16_t *v0 = v_lds + 16 * (i / DT) * D + tr_off + ((4 * (i % DT) + tr_chunk) ^ v_swizzle<D>(tr_key)) * 8;
         const uint2 lo = read_tr16(v0), hi = read_tr16(v0 + 8 * D);
-        vf[i % AHEAD] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        vf[i % kReadAhead] = make_uint4(lo.x, lo.y, hi.x, hi.y);
       };
       if constexpr (PIPE) {
         // The next tile's scores beside this one's softmax (of the last tile: of whatever the
-        // stage holds, and not used), each operand read AHEAD of its product; the order is
+        // stage holds, and not used), each operand read kReadAhead products early; the order is
         // the source's.
         const float mc = m_run * c2 - kBias;
         float ps0 = 0.0f, ps1 = 0.0f, even = 0.0f;
@@ -530,16 +530,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
 #pragma unroll
           for (int r = 0; r < 16; ++r) nx[mt][r] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < AHEAD; ++c) read_k(c);
+        for (int c = 0; c < kReadAhead; ++c) read_k(c);
 #pragma unroll
         for (int c = 0; c < MT * DC; ++c) {
           // One product, the read of a later one's operand, and one of the tile's 16 MT weights.
           static_assert(DC == 16 || !PIPE, "a weight per product");
           const int mt = c / DC, r = c % 16;
           __builtin_amdgcn_sched_barrier(0);
-          nx[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(kf[c % AHEAD]), qop[c % DC], nx[mt], 0, 0, 0);
-          if (c + AHEAD < MT * DC) read_k(c + AHEAD);
-          else read_v(c + AHEAD - MT * DC);
+          nx[mt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(kf[c % kReadAhead]), qop[c % DC], nx[mt], 0, 0, 0);
+          if (c + kReadAhead < MT * DC) read_k(c + kReadAhead);
+          else read_v(c + kReadAhead - MT * DC);
           const float e = exp2_raw(fmaf(s[mt][r], c2, -mc));
           if (r & 1) {
             pw[mt][r >> 1] = pack_f16x2(even, e);
@@ -553,6 +553,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
       } else {
         weights(m_run * c2 - kBias);
       }
+      // The reference moves only when a weight leaves f16's range: the sum is then +inf
+      // or NaN, as it is for a row without a reference yet (m_run = -inf).
       if (__any(!(psum <= __FLT_MAX__))) {
         float mx = -INFINITY;
 #pragma unroll
@@ -579,8 +581,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
           const int mt = i / DT >> 1, base = (i / DT & 1) * 4;
           const h8_t pb = as_h8(make_uint4(pw[mt][base], pw[mt][base + 1], pw[mt][base + 2], pw[mt][base + 3]));
           __builtin_amdgcn_sched_barrier(0);
-          o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(vf[i % AHEAD]), pb, o[i % DT], 0, 0, 0);
-          if (i + AHEAD < BN / 16 * DT) read_v(i + AHEAD);
+          o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(vf[i % kReadAhead]), pb, o[i % DT], 0, 0, 0);
+          if (i + kReadAhead < BN / 16 * DT) read_v(i + kReadAhead);
         }
         __builtin_amdgcn_sched_barrier(0);
       } else {
