@@ -962,3 +962,81 @@ def test_decode_of_many_short_units(ctx, hq, hkv, d, size, batch, low, high):
     got = decode(ctx, cache, q, hq)
     hold(got, *decode_want(cache, q), f"decode {batch} x {hkv}")
     assert np.array_equal(got, decode(ctx, cache, q, hq)), "two calls differ"
+
+
+@pytest.mark.parametrize("hq,hkv", [(4096, 4096), (4200, 4200), (130, 1), (1030, 103)])
+def test_many_heads(ctx, hq, hkv):
+    """As many KV heads as a decode launch takes, more than the pieces' counters reach (packed
+    rows only), and groups that are no multiple of a chunk; a sample of the heads is checked."""
+    rng = np.random.default_rng(81)
+    d, size, counts = 32, 16, [3, 0, 70]
+    starts = starts_of(counts)
+    n = int(starts[-1])
+    heads = np.unique(np.concatenate([[0, hq - 1], rng.integers(0, hq, 6)]))
+    kv = heads // (hq // hkv)
+    q, k, v = (rng.standard_normal((n, h, d)).astype(np.float16) for h in (hq, hkv, hkv))
+    cfg = AttentionConfig(hq, hkv, d)
+    batch = ctx.begin_batch()
+    out = batch.attention_packed(*[ctx.tensor(x.view(np.uint16)) for x in (q, k, v)], ctx.tensor(starts, U32), cfg)
+    batch.finish()
+    hold(ctx.download(out)[:, heads], *packed_want(q[:, heads], k[:, kv], v[:, kv], starts, True), "packed")
+    if hkv > 4096:
+        return
+    cache = Cache(ctx, rng, [130, 0, 33], 9, size, hkv, d)
+    q = rng.standard_normal((3, hq, d)).astype(np.float16)
+    got = decode(ctx, cache, q, hq)[:, heads]
+    cache.rows = [(k[:, kv], v[:, kv]) for k, v in cache.rows]
+    hold(got, *decode_want(cache, q[:, heads]), "decode")
+
+
+def test_one_graph_for_every_division_of_the_work(ctx):
+    """Captured once, replayed on lengths and row offsets that the kernels divide in every way
+    (none, short, equal, ragged, one long), each time as the eager call on them."""
+    rng = np.random.default_rng(91)
+    hq, hkv, d, size, b, n = 16, 8, 64, 16, 80, 300
+    cache = Cache(ctx, rng, [1500] * b, 94, size, hkv, d)
+    pages = (cache.key_pages, cache.value_pages, cache.device_table, cache.device_lengths)
+    one = ctx.tensor(rng.standard_normal((b, hq, d)).astype(np.float16).view(np.uint16))
+    q, k, v = (ctx.tensor(rng.standard_normal((n, h, d)).astype(np.float16).view(np.uint16)) for h in (hq, hkv, hkv))
+    dev_starts = ctx.tensor(np.zeros(b + 1, np.uint32), U32)
+    cfg = AttentionConfig(hq, hkv, d)
+
+    def enqueue(batch, outs):
+        batch.attention_decode_paged(one, *pages, cfg, out=outs[0])
+        batch.attention_paged(q, *pages, dev_starts, cfg, out=outs[1])
+        batch.attention_packed(q, k, v, dev_starts, cfg, out=outs[2])
+
+    def outputs():
+        return [ctx.tensor(np.full(t.shape, 0x1234, np.uint16)) for t in (one, q, q)]
+
+    captured = outputs()
+    batch = ctx.begin_capture()
+    enqueue(batch, captured)
+    graph = batch.end_capture()
+    ragged = rng.integers(0, 1501, b)
+    one_long = np.where(np.arange(b) == 7, 1500, 3)
+    few = np.where(np.arange(b) < 4, 1500, 0)
+    rows = {"none": np.zeros(b, int), "one": np.where(np.arange(b) == 7, n, 0), "each": np.full(b, 3),
+            "some": np.where(np.arange(b) % 11 == 0, 30, 0)}
+    for lengths, counts in ((np.zeros(b, int), "none"), (np.full(b, 20), "each"), (np.full(b, 1500), "each"),
+                            (ragged, "some"), (one_long, "one"), (few, "one"), (np.full(b, 300), "some"),
+                            (ragged, "each")):
+        ctx.upload(cache.device_lengths, lengths.astype(np.uint32))
+        ctx.upload(dev_starts, starts_of(rows[counts]))
+        for t in captured:
+            ctx.upload(t, np.full(t.shape, 0x1234, np.uint16))
+        graph.launch()
+        ctx.synchronize()
+        eager = outputs()
+        batch = ctx.begin_batch()
+        enqueue(batch, eager)
+        batch.finish()
+        for t, e in zip(captured, eager):
+            assert np.array_equal(ctx.download(t), ctx.download(e)), counts
+        got = ctx.download(captured[0])
+        for i in rng.integers(0, b, 3):
+            key, value = cache.rows[i]
+            want, tol = attend(f16(ctx.download(one))[i:i + 1].astype(np.float64), key, value,
+                               [np.arange(int(lengths[i]))], False)
+            hold(got[i:i + 1], want, tol)
+    graph.destroy()
