@@ -136,10 +136,14 @@ __device__ __forceinline__ bool plan_piece(const PackedParams &p, uint32_t rank,
     const uint32_t slots = all < p.share ? p.share - all / 2 : p.share;
     cap = max(max(kLeastPiece, (work + slots - 1) / slots), (most + kMostPieces - 1) / kMostPieces);
   }
-  // The cut tiles: those of at least cap + 1 key tiles, sequence after sequence.
+  // The cut tiles: those of at least cap + 1 key tiles, sequence after sequence. Should they
+  // come to more than max_pieces, again with longer ones, once every wave is past its reads
+  // of s_before.
   uint32_t cuts = 0, pieces = 0;
-  bool found = false;
+  bool found = false, again = false;
   for (;; cap *= 2) {
+    if (again) __syncthreads();
+    again = true;
     cuts = pieces = 0;
     found = false;
     if (cap >= most) break;
