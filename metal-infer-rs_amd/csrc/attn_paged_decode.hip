@@ -42,6 +42,8 @@ constexpr uint32_t kPiece = kWaves, kShare = 2;
 // unit's are joined in steps of kJoin.
 constexpr uint32_t kUneven = 2, kJoin = 16;
 constexpr uint32_t kJoinTiles = 12;  // tiles that take as long as shares' partials and joins
+// The least weight of a part in a join: nothing beside finite sums, but not 0.
+constexpr float kSmallest = 0x1p-126f;
 
 __device__ __forceinline__ float lane_value(float x, int lane) {
   return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), lane));
@@ -172,8 +174,9 @@ __device__ __forceinline__ void join_parts(float *partial, size_t row_stride, ui
 #pragma unroll
       for (uint32_t h = 0; h < HEADS; ++h) {
         const float m = fmaxf(M[h], max32((uint32_t)lane < n ? ml[h].x : -INFINITY));
-        // -inf: a part of which no key has a page.
-        const float f = (uint32_t)lane >= n || ml[h].x == -INFINITY ? 0.0f : exp2_raw((ml[h].x - m) * scale_log2);
+        // A part without a weight (no key of it has a page) is left out. One whose scores are all
+        // NaN has no maximum either, but its sum is NaN, and any weight above zero keeps that.
+        const float f = (uint32_t)lane >= n || ml[h].y == 0.0f ? 0.0f : fmaxf(exp2_raw((ml[h].x - m) * scale_log2), kSmallest);
         const float r = M[h] == -INFINITY ? 0.0f : exp2_raw((M[h] - m) * scale_log2);
         M[h] = m;
         L[h] = fmaf(L[h], r, sum32(f != 0.0f ? ml[h].y * f : 0.0f));
