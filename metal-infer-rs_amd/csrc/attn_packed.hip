@@ -778,8 +778,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
             for (int i = 0; i < 16; ++i) acc[u][i] *= r;
 #pragma unroll
             for (uint32_t k = 0; k < FEW; ++k) {
-              // -inf: a piece in which the row saw no key.
-              const bool use = s0 + k < parts && ml[u][k].x != -INFINITY;
+              // A sum of 0: a piece in which the row saw no key. (One whose scores are all NaN has
+              // no maximum either, but a NaN sum.)
+              const bool use = s0 + k < parts && ml[u][k].y != 0.0f;
               const float f = use ? exp2_raw((ml[u][k].x - m) * c2) : 0.0f;
               sum[u] = use ? fmaf(ml[u][k].y, f, sum[u]) : sum[u];
 #pragma unroll
