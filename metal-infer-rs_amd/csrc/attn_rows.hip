@@ -1151,9 +1151,11 @@ __global__ __launch_bounds__(1024) void attn_stream_merge_kernel(const RowsParam
     // hold other data).
     auto fold = [&](auto n_tag, uint32_t left) __attribute__((always_inline)) {
       constexpr int N = decltype(n_tag)::value;
+      // A piece without a weight has the sum 0; one whose scores are all NaN has no maximum
+      // either, but a NaN sum, which the weight 0 keeps.
       bool use[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) use[i] = (uint32_t)i < left && m[i] != -INFINITY;
+      for (int i = 0; i < N; ++i) use[i] = (uint32_t)i < left && l[i] != 0.0f;
       float cm = M;
 #pragma unroll
       for (int i = 0; i < N; ++i) cm = use[i] ? fmaxf(cm, m[i]) : cm;
