@@ -380,7 +380,7 @@ __global__ __launch_bounds__(256) void attn_tiled_merge_kernel(const PrefillPara
     float cm = M;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      if (s0 + i >= nsplits) ml[i].x = -INFINITY;
+      if (s0 + i >= nsplits) ml[i] = make_float2(-INFINITY, 0.0f);
       cm = fmaxf(cm, ml[i].x);
     }
     const float alpha = M == -INFINITY ? 0.0f : exp2_raw(M - cm);
@@ -388,7 +388,9 @@ __global__ __launch_bounds__(256) void attn_tiled_merge_kernel(const PrefillPara
     acc *= alpha;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      if (ml[i].x == -INFINITY) continue;
+      // A sum of 0: a split in which the row saw no key. (One whose scores are all NaN has
+      // no maximum either, but a NaN sum.)
+      if (ml[i].y == 0.0f) continue;
       const float f = exp2_raw(ml[i].x - cm);
       L = fmaf(ml[i].y, f, L);
 #pragma unroll

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import mi_attn
-from helpers import f16, oracle_attention, run_attention
+from helpers import f16, oracle_attention, run_attention, upload_kv
 
 pytestmark = pytest.mark.gpu
 NAN = np.float16(np.nan).view(np.uint16)
@@ -37,6 +37,21 @@ def test_batched_decode_nan_in_the_newest_key(ctx, hq, hkv, d, cap, lengths):
     n = lengths[-1]
     ref = oracle_attention(q[-1:], k[-1, :n], v[-1, :n], hq=hq, hkv=hkv, d=d, off=n - 1)["f32"]
     assert np.abs(got[-1:] - ref).max() <= 2e-3
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("T,off", [(24, 1100), (31, 20000), (300, 700)])
+def test_tiled_nan_in_every_key_of_some_splits(ctx, d, T, off):
+    hq, hkv, L = 8, 1, off + T
+    q, k, v = rand(4, (T, hq, d)), rand(5, (L, hkv, d)), rand(6, (L, hkv, d))
+    cfg = mi_attn.AttentionConfig(hq, hkv, d, True, off)
+    _, view = upload_kv(ctx, k, "head_major")
+    info = ctx.plan(ctx.tensor(q), view, view, cfg, mi_attn.TILED)
+    assert info["kernel"] == "attn_tiled" and info["splits"] > 1, info
+    block = info["block_keys"]
+    k[block:2 * block] = NAN
+    got = f16(run_attention(ctx, q, k, v, hq=hq, hkv=hkv, d=d, off=off, kind="tiled"))
+    assert np.isnan(got).all()
 
 
 @pytest.mark.parametrize("d", [64, 128])
