@@ -42,8 +42,19 @@ constexpr uint32_t kPiece = kWaves, kShare = 2;
 // unit's are joined in steps of kJoin.
 constexpr uint32_t kUneven = 2, kJoin = 16;
 constexpr uint32_t kJoinTiles = 12;  // tiles that take as long as shares' partials and joins
-// The least weight of a part in a join: nothing beside finite sums, but not 0.
+// The least weight of a part in a join, and the least rescaling factor: nothing beside finite
+// sums, but not 0, so that an infinity far below the other keys stays one.
 constexpr float kSmallest = 0x1p-126f;
+
+// Two f16 that are not negative, or f16's smallest value where one is zero.
+__device__ __forceinline__ uint32_t above_zero(uint32_t w) {
+  typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, w), u16x2_t{1, 1}));
+}
+// The two values of a pair over the row's sum: of a row without a weight above zero 0 / 0.
+__device__ __forceinline__ uint32_t over_sum(float a, float b, float sum) {
+  return sum == 0.0f ? 0x7e007e00u : pack_f16x2(a / sum, b / sum);
+}
 
 __device__ __forceinline__ float lane_value(float x, int lane) {
   return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), lane));
@@ -174,10 +185,10 @@ __device__ __forceinline__ void join_parts(float *partial, size_t row_stride, ui
 #pragma unroll
       for (uint32_t h = 0; h < HEADS; ++h) {
         const float m = fmaxf(M[h], max32((uint32_t)lane < n ? ml[h].x : -INFINITY));
-        // A part without a weight (no key of it has a page) is left out. One whose scores are all
-        // NaN has no maximum either, but its sum is NaN, and any weight above zero keeps that.
-        const float f = (uint32_t)lane >= n || ml[h].y == 0.0f ? 0.0f : fmaxf(exp2_raw((ml[h].x - m) * scale_log2), kSmallest);
-        const float r = M[h] == -INFINITY ? 0.0f : exp2_raw((M[h] - m) * scale_log2);
+        // A part without a maximum has a sum of 0 (no key with a page) or of NaN (every score
+        // is), which any weight above zero keeps.
+        const float f = (uint32_t)lane >= n ? 0.0f : fmaxf(exp2_raw((ml[h].x - m) * scale_log2), kSmallest);
+        const float r = fmaxf(exp2_raw((M[h] - m) * scale_log2), kSmallest);
         M[h] = m;
         L[h] = fmaf(L[h], r, sum32(f != 0.0f ? ml[h].y * f : 0.0f));
         if ((uint32_t)lane < MOST) s_f[h * FROW + lane] = f;
@@ -207,9 +218,8 @@ __device__ __forceinline__ void join_parts(float *partial, size_t row_stride, ui
       const uint32_t i = i0 + 64 * u + lane;
       const float sum = s_f[hd[u] * FROW + MOST + 1];
       if (i >= pairs) continue;
-      if (out != nullptr)  // no key with a page: 0 / 0
-        *reinterpret_cast<uint32_t *>(out + i / (D / 2) * o_head + i % (D / 2) * 2) =
-            pack_f16x2(A[u].x / sum, A[u].y / sum);
+      if (out != nullptr)
+        *reinterpret_cast<uint32_t *>(out + i / (D / 2) * o_head + i % (D / 2) * 2) = over_sum(A[u].x, A[u].y, sum);
       else
         store_partial2(partial + at[u], A[u].x, A[u].y);
     }
@@ -241,10 +251,10 @@ __global__ __launch_bounds__(kWaves * 64, per_cu(D)) void attn_decode_paged_kern
   constexpr uint32_t HELD = 32, ROW = D + 2;  // tiles whose page ids a wave holds; floats of a partial's head
   // Added to every weight's exponent, so that the low terms stay above f16's smallest
   // values; it cancels between the weighted sum and the row sum. The high terms round
-  // towards zero, and the low ones get kLeast, f16's smallest value (2^-37 of the largest
-  // weight): neither is negative and one is above zero, so that an infinity that a row
-  // sees stays one.
-  constexpr float kBias = 13.0f, kGrow = 2.0f, kLeast = 0x1p-24f;
+  // towards zero, so that the low ones are not negative either, and a term of 0 becomes
+  // f16's smallest value (2^-37 of the largest weight): 0 times an infinity that the row
+  // sees would be NaN.
+  constexpr float kBias = 13.0f, kGrow = 2.0f;
   // A stage of V per wave; the waves' rows once a piece's tiles are done.
   __shared__ __attribute__((aligned(16))) uint16_t v_lds[WAVES * STAGE];
   __shared__ float s_m[WAVES][GM], s_l[WAVES][GM];
@@ -423,7 +433,7 @@ __global__ __launch_bounds__(kWaves * 64, per_cu(D)) void attn_decode_paged_kern
       // the first tile), which keeps P at 2^15 or less.
       if (__any((mx - m_run) * c2 > kGrow)) {
         const float m_new = fmaxf(m_run, mx);
-        const float alpha = m_new == -INFINITY ? 1.0f : exp2_raw((m_run - m_new) * c2);
+        const float alpha = m_new == -INFINITY ? 1.0f : fmaxf(exp2_raw((m_run - m_new) * c2), kSmallest);
         l_run *= alpha;
 #pragma unroll
         for (int dt = 0; dt < DB; ++dt) o[dt] *= alpha;
@@ -437,8 +447,8 @@ __global__ __launch_bounds__(kWaves * 64, per_cu(D)) void attn_decode_paged_kern
         for (int e = 0; e < 4; e += 2) {
           const float w0 = exp2_raw(fmaf(s[hf][e], c2, -mc)), w1 = exp2_raw(fmaf(s[hf][e + 1], c2, -mc));
           const uint32_t wv = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(w0, w1));
-          pw[2 * hf + e / 2] = wv;
-          pl[2 * hf + e / 2] = pack_f16x2(w0 - lo_f16(wv) + kLeast, w1 - hi_f16(wv) + kLeast);
+          pw[2 * hf + e / 2] = above_zero(wv);
+          pl[2 * hf + e / 2] = above_zero(pack_f16x2(w0 - lo_f16(wv), w1 - hi_f16(wv)));
           l_run += w0 + w1;
         }
       const h8_t hi_p = as_h8(make_uint4(pw[0], pw[1], pw[2], pw[3]));
@@ -481,8 +491,8 @@ __global__ __launch_bounds__(kWaves * 64, per_cu(D)) void attn_decode_paged_kern
         const uint32_t g = i / (D / 2), d = i % (D / 2) * 2;
         const float2 v = *reinterpret_cast<const float2 *>(rows + 2 * i);
         const float l = s_l[wave][g];
-        if (pieces == 1) {  // no key with a page: 0 / 0
-          *reinterpret_cast<uint32_t *>(out + g * o_head + d) = pack_f16x2(v.x / l, v.y / l);
+        if (pieces == 1) {
+          *reinterpret_cast<uint32_t *>(out + g * o_head + d) = over_sum(v.x, v.y, l);
         } else {
           store_partial2(partial + g * ROW + 2 + d, v.x, v.y);
           if (d == 0) store_partial2(partial + g * ROW, s_m[wave][g], l);
@@ -506,14 +516,14 @@ __global__ __launch_bounds__(kWaves * 64, per_cu(D)) void attn_decode_paged_kern
         float L = 0.0f, A0 = 0.0f, A1 = 0.0f;
 #pragma unroll
         for (int v = 0; v < WAVES; ++v) {
-          const float f = s_m[v][g] == -INFINITY ? 0.0f : exp2_raw((s_m[v][g] - M) * c2);
+          const float f = fmaxf(exp2_raw((s_m[v][g] - M) * c2), kSmallest);  // as in a join
           const float2 x = *reinterpret_cast<const float2 *>(s_o + (v * GM + g) * D + d);
           L += s_l[v][g] * f;
           A0 += x.x * f;
           A1 += x.y * f;
         }
         if (pieces == 1) {
-          *reinterpret_cast<uint32_t *>(out + g * o_head + d) = pack_f16x2(A0 / L, A1 / L);
+          *reinterpret_cast<uint32_t *>(out + g * o_head + d) = over_sum(A0, A1, L);
         } else {
           store_partial2(partial + g * ROW + 2 + d, A0, A1);
           if (d == 0) store_partial2(partial + g * ROW, M, L);

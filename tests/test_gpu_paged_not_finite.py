@@ -105,3 +105,81 @@ def test_packed_nan_in_every_key_of_the_last_pieces(ctx, d, causal):
         got = packed(ctx, q, bad, v, starts_of([n]), causal)
         at = first if causal else 0
         assert np.isfinite(got[:at]).all() and np.isnan(got[at:]).all(), f"from key {first}"
+
+
+# -------------------------------------------------- infinities of small weights --
+
+def far(rng, n, hq, hkv, d, seen, gap):
+    """q, k, v of n keys of which those of `seen` have scores `gap` below the others'."""
+    q, k, v = (rng.standard_normal((n, h, d)).astype(np.float16) for h in (hq, hkv, hkv))
+    q[:, :, 0], k[:, :, 0] = 8, 0
+    k[seen, :, 0] = -gap * np.sqrt(d) / 8
+    return q, k, v
+
+
+GAPS = [25.0, 60.0, 200.0]  # weights of 2^-36, 2^-87 and 2^-289 of the largest
+
+
+def check_infinite(got, lim, at):
+    """Rows got [n, H, D], which see keys up to lim[i]: columns 3 to 6."""
+    for key, what, col in ((at[0], np.inf, 3), (at[1], -np.inf, 4)):
+        sees = lim >= key
+        assert (got[sees][..., col] == what).all() and np.isfinite(got[~sees][..., col]).all()
+    sees = lim >= at[2]
+    assert np.isnan(got[sees][..., 5]).all() and np.isfinite(got[~sees][..., 5]).all()
+    both, one = lim >= max(at[0], at[1]), (lim >= min(at[0], at[1])) & (lim < max(at[0], at[1]))
+    assert np.isnan(got[both][..., 6]).all() and np.isinf(got[one][..., 6]).all()
+    rest = [c for c in range(got.shape[-1]) if not 3 <= c <= 6]
+    assert np.isfinite(got[..., rest]).all()
+
+
+def put_infinite(v, at):
+    v[at[0], :, 3], v[at[1], :, 4], v[at[2], :, 5] = np.inf, -np.inf, np.nan
+    v[at[0], :, 6], v[at[1], :, 6] = np.inf, -np.inf
+
+
+@pytest.mark.parametrize("gap", GAPS)
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("keys,batch,hkv", [(90, 1, 1), (4000, 1, 2), (333, 70, 16), (40, 70, 16)])
+def test_decode_infinities_of_small_weights(ctx, d, keys, batch, hkv, gap):
+    """One piece, pieces of workgroups, shares of waves and whole units."""
+    rng = np.random.default_rng(d + keys)
+    at = [keys // 2, 3, keys - 2]
+    q, k, v = far(rng, keys, hkv, hkv, d, at, gap)
+    put_infinite(v, at)
+    lengths = [keys] * batch
+    if batch > 60:
+        lengths[5], lengths[9] = 3 * keys, 0
+    cache = Cache(ctx, rng, lengths, -(-max(lengths) // 16), 16, hkv, d)
+    for i in range(batch):
+        if lengths[i] == keys:
+            cache.rows[i] = (k, v)
+    stored(cache)
+    got = f16(decode(ctx, cache, np.repeat(q[:1], batch, 0), hkv))
+    for i in range(batch):
+        if lengths[i] == keys:
+            check_infinite(got[i:i + 1], np.array([keys - 1]), at)
+    if batch > 60:
+        assert np.isfinite(got[5]).all() and np.isnan(got[9]).all()
+
+
+# ---------------------------------------------------------- no finite score at all --
+
+def without_scores(ctx, d, lengths, hkv=1):
+    """A cache whose keys are -inf where the queries are 1, but for the last sequence's."""
+    rng = np.random.default_rng(d)
+    cache = Cache(ctx, rng, lengths, -(-max(lengths) // 16), 16, hkv, d)
+    for k, _ in cache.rows[:-1]:
+        k[:, :, 0] = -np.inf
+    q = rng.standard_normal((len(lengths), 2 * hkv, d)).astype(np.float16)
+    q[:, :, 0] = 1
+    return stored(cache), q
+
+
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("lengths,hkv", [([1, 40, 3000, 20], 1), ([1, 40, 0, 120] * 30 + [70], 8), ([900, 1, 40] * 20 + [70], 16)])
+def test_decode_rows_whose_scores_are_all_minus_infinity(ctx, d, lengths, hkv):
+    """The weights of such a row are 0 / 0."""
+    cache, q = without_scores(ctx, d, lengths, hkv)
+    got = f16(decode(ctx, cache, q, 2 * hkv))
+    assert np.isnan(got[:-1]).all() and np.isfinite(got[-1]).all()
