@@ -380,7 +380,7 @@ __global__ __launch_bounds__(256) void attn_tiled_merge_kernel(const PrefillPara
     float cm = M;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      if (s0 + i >= nsplits) ml[i] = make_float2(-INFINITY, 0.0f);
+      if (s0 + i >= nsplits) ml[i].x = -INFINITY;
       cm = fmaxf(cm, ml[i].x);
     }
     const float alpha = M == -INFINITY ? 0.0f : exp2_raw(M - cm);
@@ -388,10 +388,10 @@ __global__ __launch_bounds__(256) void attn_tiled_merge_kernel(const PrefillPara
     acc *= alpha;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      // A sum of 0: a split in which the row saw no key. (One whose scores are all NaN has
-      // no maximum either, but a NaN sum.)
-      if (ml[i].y == 0.0f) continue;
-      const float f = exp2_raw(ml[i].x - cm);
+      if (s0 + i >= nsplits) continue;
+      // Of a split without a maximum 0: its sum is 0 (the row saw no key), or NaN (every
+      // score is), which stays.
+      const float f = fmaxf(exp2_raw(ml[i].x - cm), 0.0f);
       L = fmaf(ml[i].y, f, L);
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] = fmaf(a[i][e], f, acc[e]);
