@@ -57,6 +57,8 @@ constexpr uint32_t kLeastPiece = 8, kMostPieces = 32;
 // a tile: 48 us by one workgroup each, 42 us four at a time.)
 constexpr uint32_t kOneJoin = 8;
 __device__ __forceinline__ uint32_t join_size(uint32_t pieces) { return pieces > 16 ? 6 : 4; }
+// The least weight of a piece in a join: nothing beside finite sums, but not 0.
+constexpr float kSmallest = 0x1p-126f;
 constexpr int kReadAhead = 4;       // LDS operand reads in flight ahead of the MFMAs
 constexpr int kSchedMfma = 0x008, kSchedDsRead = 0x100;
 
@@ -243,8 +245,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   // tell the loads into one from the reads of the other.
   __shared__ __attribute__((aligned(16))) uint16_t k_lds_a[OUT], k_lds_b[OUT];
   __shared__ __attribute__((aligned(16))) uint16_t v_lds_a[TILE], v_lds_b[TILE];
-  // s_bad[st] = ti + 1: V of the masked tile ti in stage st holds a value that is not finite.
-  __shared__ uint32_t s_bad[2];
+  __shared__ uint32_t s_bad;  // whether some of the piece's V decide columns whatever their weights are
   __shared__ Rows s_rows[kPackedMaxBatch];
   __shared__ uint32_t s_before[kPackedMaxBatch + 1], s_last;
   auto k_stage = [&](int st) __attribute__((always_inline)) -> uint16_t * { return st ? k_lds_b : k_lds_a; };
@@ -369,7 +370,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   const uint32_t n_full = full_lim < 0 ? 0 : (uint32_t)min((int64_t)t_end, (full_lim + 1) / BN);
   // A masked tile's V may hold values that some of its rows must not see and that are
   // not finite, and 0 times those is NaN. Each wave looks at the rows it has loaded: such
-  // values become zeros, and the rows that see them get them from memory (add_bad).
+  // values become zeros, and the rows that see them get them after the last tile.
   auto look = [&](uint32_t ti, int stage) __attribute__((always_inline)) {
     if (ti < n_full) return;
     uint16_t *mine = v_stage(stage) + wave * RPW * D;
@@ -383,7 +384,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
         bad = true;
       }
     }
-    if (__any(bad)) s_bad[stage] = ti + 1;
+    if (__any(bad)) s_bad = 1;
   };
 
   float16_t o[DT];
@@ -399,36 +400,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   const int tr_key = 4 * (tr_g >> 1) + tr_j;
   const int tr_off = tr_key * D + 4 * (tr_a & 1);
   const int tr_chunk = 2 * (tr_g & 1) + (tr_a >> 1);
-
-  // Adds the values of the tile at key j0 that are not finite to the rows that see them (a
-  // positive weight leaves an infinity or NaN what it is).
-  auto add_bad = [&](uint32_t j0) __attribute__((always_inline)) {
-#pragma unroll 1
-    for (uint32_t key = j0; key < min(j0 + BN, kmax); ++key) {
-      const uint16_t *row = p.kv.v + (int64_t)kvh * p.kv.v_head;
-      if constexpr (PAGED) {
-        const uint32_t page = p.kv.table[(int64_t)b * p.kv.table_seq + (key >> shift)];
-        if (page >= p.kv.pages) continue;
-        row += (int64_t)page * p.kv.v_page + (int64_t)(key & in_page) * p.kv.v_pos;
-      } else {
-        row += (int64_t)(range.begin + key) * p.kv.v_pos;
-      }
-      if ((int64_t)key > lim) continue;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          // d = 32 dt + 8 q + 4 h + e of this lane's row.
-          const uint2 v = *reinterpret_cast<const uint2 *>(row + 32 * dt + 8 * q + 4 * h);
-          const uint32_t w[2] = {v.x, v.y};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint16_t x = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-            if ((x & 0x7c00u) == 0x7c00u) o[dt][4 * q + e] += f16_to_f32(x);
-          }
-        }
-    }
-  };
 
   float16_t s_cur[MT];  // with PIPE: the scores of the tile that the next step takes
   // S^T[key][row] = K Q^T of a tile.
@@ -611,9 +582,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
         __builtin_amdgcn_sched_group_barrier(kSchedMfma, kReadAhead, 1);
         __builtin_amdgcn_s_setprio(0);
       }
-      if constexpr (MASK) {
-        if (s_bad[ST] == it + 1) add_bad(j0);
-      }
       if constexpr (PIPE) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) s_cur[mt] = nx[mt];
@@ -636,7 +604,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   };
 
   if (t_begin < t_end) {
-    if (tid < 2) s_bad[tid] = 0;
+    if (tid == 0) s_bad = 0;
     __syncthreads();
     if constexpr (PIPE) {
       find(t_begin);
@@ -687,6 +655,62 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   }
 
   const float l_total = l_run + __shfl_xor(l_run, 32, 64);
+  if (t_begin < t_end) {
+    // A weight below f16's smallest value is 0, and 0 times an infinity that the row sees is
+    // NaN, where the weight itself leaves the infinity. Where a row with a finite sum has a
+    // value that is not finite, or a masked tile's were taken out, the workgroup looks at
+    // the values of its keys again: a column's infinities and NaN decide it.
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // one chain of additions would take 0.2 us
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum[r & 3] = fmaf(o[dt][r], 0.0f, sum[r & 3]);
+    if (__any(sum[0] + sum[1] + sum[2] + sum[3] != 0.0f && l_total > 0.0f)) s_bad = 1;
+    __syncthreads();  // also: every wave is past its last LDS operand read
+    if (s_bad != 0) {
+      // The first keys of each column that hold an infinity or NaN, and a negative one or NaN.
+      uint32_t *first = reinterpret_cast<uint32_t *>(k_lds_a);
+      for (uint32_t i = tid; i < 2 * D; i += 256) first[i] = ~0u;
+      __syncthreads();
+      const uint32_t last = min(t_end * BN, kmax), chunk = lane % CPR;
+#pragma unroll 1
+      for (uint32_t key = t_begin * BN + 16 * wave; key < last; key += 64) {
+        const uint16_t *row = p.kv.v + (int64_t)kvh * p.kv.v_head + 8 * chunk;
+        bool there = true;
+        if constexpr (PAGED) {
+          const uint32_t page = p.kv.table[(int64_t)b * p.kv.table_seq + (key >> shift)];
+          there = page < p.kv.pages;
+          row += (int64_t)page * p.kv.v_page + (int64_t)(key & in_page) * p.kv.v_pos;
+        } else {
+          row += (int64_t)(range.begin + key) * p.kv.v_pos;
+        }
+#pragma unroll
+        for (int i = 0; i < CPR / 4; ++i) {
+          const uint32_t r = (64 * i + lane) / CPR;
+          if (!there || key + r >= last) continue;
+          uint32_t bits = not_finite_columns(*reinterpret_cast<const uint4 *>(row + (int64_t)r * p.kv.v_pos));
+          for (uint32_t e = 0; bits != 0; ++e, bits >>= 2) {
+            if ((bits & 1) != 0) atomicMin(&first[8 * chunk + e], key + r);
+            if ((bits & 2) != 0) atomicMin(&first[D + 8 * chunk + e], key + r);
+          }
+        }
+      }
+      __syncthreads();
+      if (l_total > 0.0f) {
+        // d = 32 dt + 8 q + 4 h + e of this lane's row, which sees the keys up to lim.
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const uint32_t d = 32 * dt + 8 * (r >> 2) + 4 * h + (r & 3);
+            const bool positive = (int64_t)first[d] <= lim, negative = (int64_t)first[D + d] <= lim;
+            if (positive) o[dt][r] = negative ? __builtin_nanf("") : INFINITY;
+            else if (negative) o[dt][r] = -INFINITY;
+          }
+      }
+      __syncthreads();
+    }
+  }
   const uint32_t pieces = __builtin_amdgcn_readfirstlane(pc.pieces), piece = __builtin_amdgcn_readfirstlane(pc.piece);
   // 32 rows of each wave as f16, in a region of the idle stages.
   auto rows_lds = [&](int v) __attribute__((always_inline)) { return (v < 2 ? k_lds_a : k_lds_b) + (v & 1) * 32 * D; };
@@ -771,17 +795,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
             float m = M[u];
 #pragma unroll
             for (uint32_t k = 0; k < FEW; ++k) m = s0 + k < parts ? fmaxf(m, ml[u][k].x) : m;
-            const float r = M[u] == -INFINITY ? 0.0f : exp2_raw((M[u] - m) * c2);
+            // Never 0, so that an infinity of a piece far below the others stays one. A piece
+            // without a maximum has a sum of 0 (the row saw no key) or of NaN (every score is).
+            const float r = fmaxf(exp2_raw((M[u] - m) * c2), kSmallest);
             M[u] = m;
             sum[u] *= r;
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[u][i] *= r;
 #pragma unroll
             for (uint32_t k = 0; k < FEW; ++k) {
-              // A sum of 0: a piece in which the row saw no key. (One whose scores are all NaN has
-              // no maximum either, but a NaN sum.)
-              const bool use = s0 + k < parts && ml[u][k].y != 0.0f;
-              const float f = use ? exp2_raw((ml[u][k].x - m) * c2) : 0.0f;
+              const bool use = s0 + k < parts;
+              const float f = fmaxf(exp2_raw((ml[u][k].x - m) * c2), kSmallest);
               sum[u] = use ? fmaf(ml[u][k].y, f, sum[u]) : sum[u];
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
@@ -818,7 +842,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
   constexpr int RPI = 64 / CPR;  // rows per store instruction
   if (!join) {
     const float inv = 1.0f / l_total;
-    __syncthreads();  // every wave is past its last LDS operand read
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll

@@ -79,6 +79,19 @@ __device__ __forceinline__ uint32_t divide(uint32_t x, kernels::Divisor d) {
   return (uint32_t)(((uint64_t)x * d.magic) >> d.shift);
 }
 
+// Of the eight f16 of `v`: bit 2 e where element e is an infinity or NaN and not negative, bit
+// 2 e + 1 where it is a negative one; NaN has both.
+__device__ __forceinline__ uint32_t not_finite_columns(uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t bits = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t x = w[e >> 1] >> (16 * (e & 1)) & 0xffffu, kind = (x & 0x7fffu) > 0x7c00u ? 3u : x >> 15 ? 2u : 1u;
+    bits |= (x & 0x7c00u) == 0x7c00u ? kind << 2 * e : 0u;
+  }
+  return bits;
+}
+
 // s_waitcnt vmcnt(N), the other counters left at their maxima.
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {

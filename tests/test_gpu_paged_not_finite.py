@@ -7,7 +7,7 @@ import pytest
 
 from mi_attn import U32, AttentionConfig
 from helpers import f16
-from test_gpu_paged import Cache, attend, decode, hold, paged, starts_of
+from test_gpu_paged import Cache, attend, decode, hold, packed_want, paged, starts_of
 
 pytestmark = pytest.mark.gpu
 
@@ -139,6 +139,44 @@ def put_infinite(v, at):
 
 
 @pytest.mark.parametrize("gap", GAPS)
+@pytest.mark.parametrize("d,n", [(32, 300), (64, 300), (128, 300), (256, 300), (128, 1300), (256, 1300)])
+def test_packed_infinities_of_small_weights(ctx, d, n, gap):
+    """In whole tiles, which need no mask, and in the pieces of cut row tiles (1300 rows)."""
+    rng = np.random.default_rng(d)
+    at = [70, 40, 100]
+    q, k, v = far(rng, n, 4, 2, d, at, gap)
+    put_infinite(v, at)
+    got = packed(ctx, q, k, v, starts_of([n]))
+    check_infinite(got, np.arange(n), at)
+    got = packed(ctx, q, k, v, starts_of([n]), causal=False)
+    check_infinite(got, np.full(n, n - 1), at)
+    clean = np.where(np.isfinite(v), v, np.float16(0))
+    want, tol = packed_want(q, k, clean, starts_of([n]), True)
+    rest = [c for c in range(d) if not 3 <= c <= 6]
+    got = packed(ctx, q, k, v, starts_of([n]))
+    assert (np.abs(got - want)[..., rest] <= tol[..., rest]).all()
+
+
+@pytest.mark.parametrize("gap", GAPS)
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("keys", [900, 6000])
+def test_paged_infinities_of_small_weights(ctx, d, keys, gap):
+    rng = np.random.default_rng(d + keys)
+    at = [keys // 2, 130, keys - 20]
+    q, k, v = far(rng, keys, 4, 1, d, at, gap)
+    put_infinite(v, at)
+    cache = Cache(ctx, rng, [keys, 50], keys // 16 + 1, 16, 1, d, missing=[(0, 20)])
+    cache.rows[0] = (k, v)
+    cache.rows[1][1][10:] = np.nan
+    stored(cache)
+    starts = starts_of([40, 45])
+    q = np.concatenate([q[:40], rng.standard_normal((45, 4, d)).astype(np.float16)])
+    got = f16(paged(ctx, cache, q, starts, 4))
+    check_infinite(got[:40], keys - 40 + np.arange(40), at)
+    assert np.isfinite(got[40:45]).all() and np.isnan(got[45:]).all()  # its rows see 6 to 50 keys
+
+
+@pytest.mark.parametrize("gap", GAPS)
 @pytest.mark.parametrize("d", [32, 64, 128, 256])
 @pytest.mark.parametrize("keys,batch,hkv", [(90, 1, 1), (4000, 1, 2), (333, 70, 16), (40, 70, 16)])
 def test_decode_infinities_of_small_weights(ctx, d, keys, batch, hkv, gap):
@@ -183,3 +221,10 @@ def test_decode_rows_whose_scores_are_all_minus_infinity(ctx, d, lengths, hkv):
     cache, q = without_scores(ctx, d, lengths, hkv)
     got = f16(decode(ctx, cache, q, 2 * hkv))
     assert np.isnan(got[:-1]).all() and np.isfinite(got[-1]).all()
+
+
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+def test_paged_rows_whose_scores_are_all_minus_infinity(ctx, d):
+    cache, q = without_scores(ctx, d, [1, 40, 3000, 20])
+    got = f16(paged(ctx, cache, q, starts_of([1, 1, 1, 1]), 2))
+    assert np.isnan(got[:3]).all() and np.isfinite(got[3]).all()
