@@ -413,11 +413,12 @@ mi_status mi_decode_step_attention(mi_batch *batch, const mi_tensor *q,
  *    innermost stride (storage [P, Hkv, S, D] keeps a head's keys together), S a
  *    power of two from 16 to 2^20. block_table, device u32 [B, M] (any row
  *    stride, M * S below 2^31): position p of sequence b is in page
- *    block_table[b, p / S] at p % S. An id of P or more names no page: no row sees its keys, and a row
- *    that would be stored there is not. Sequences may share pages that they only
+ *    block_table[b, p / S] at p % S. An id of P or more names no page, and a
+ *    position of M * S or more has none: no row sees its keys, and a row that
+ *    would be stored there is not. Sequences may share pages that they only
  *    read; which of two rows written to one slot stays is not defined.
  *  - lengths, device u32 [B]: keys of each sequence with the step's rows
- *    appended (values above M * S are clamped to M * S). Row i of sequence b's n
+ *    appended (mi_attention_paged takes values above M * S for M * S). Row i of sequence b's n
  *    rows has position lengths[b] - n + i, and sees keys 0 to that (all of them
  *    where config->causal is 0). A row that sees no key, as of a sequence of
  *    length 0, gets NaN (0/0); keys that a row does not see do not reach its

@@ -329,7 +329,8 @@ constexpr uint64_t tiled_partial_floats(uint64_t splits, uint64_t row_tiles, uin
 hipError_t launch_tiled(const PrefillParams &p, uint32_t head_dim, TiledPhase phase, const Launch &l);
 // Keys and values in pages: [pages, 2^page_shift, Hkv, D] views, and of each sequence
 // the pages it has (table [B, table_width], rows table_seq words apart) and its length.
-// A page id past the last page names no page: its keys are seen by no row. Within a
+// A page id past the last page names no page, and positions past the table have none: their
+// keys are seen by no row, and no row is stored there. Within a
 // page the position stride is not negative and the page spans less than 2 GiB.
 struct PagedKv {
   const uint16_t *k;

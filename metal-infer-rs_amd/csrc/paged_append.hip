@@ -60,10 +60,11 @@ __global__ __launch_bounds__(64) void paged_append_kernel(PagedAppendParams p) {
   const uint32_t b = sequence_of_row(p.row_starts, p.batch, row, lane);
   const RowRange range = sequence_rows(p.row_starts, b, p.rows);
   if (row < range.begin || row >= range.end) return;  // no sequence has this row
-  const uint32_t len = paged_length(p.kv, b), behind = range.end - row;
+  const uint32_t len = p.kv.lengths[b], behind = range.end - row;
   if (len < behind) return;  // more rows than keys: this one has no position
   const uint32_t position = len - behind, slot = position & ((1u << p.kv.page_shift) - 1);
-  const uint32_t page = p.kv.table[(int64_t)b * p.kv.table_seq + (position >> p.kv.page_shift)];
+  const uint32_t at = position >> p.kv.page_shift;  // past the table: no page
+  const uint32_t page = at < p.kv.table_width ? p.kv.table[(int64_t)b * p.kv.table_seq + at] : ~0u;
   float c[8], s[8];
   if (!is_value(0)) {
 #pragma unroll
