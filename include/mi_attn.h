@@ -418,10 +418,10 @@ mi_status mi_decode_step_attention(mi_batch *batch, const mi_tensor *q,
  *    would be stored there is not. Sequences may share pages that they only
  *    read; which of two rows written to one slot stays is not defined.
  *  - lengths, device u32 [B]: keys of each sequence with the step's rows
- *    appended (mi_attention_paged takes values above M * S for M * S). Row i of sequence b's n
- *    rows has position lengths[b] - n + i, and sees keys 0 to that (all of them
- *    where config->causal is 0). A row that sees no key, as of a sequence of
- *    length 0, gets NaN (0/0); keys that a row does not see do not reach its
+ *    appended, also where the table has no room for them. Row i of sequence b's
+ *    n rows has position lengths[b] - n + i, and sees keys 0 to that (all of
+ *    them where config->causal is 0). A row that sees no key, as of a sequence
+ *    of length 0, gets NaN (0/0); keys that a row does not see do not reach its
  *    result, whatever they hold.
  *  - head_dim 32, 64, 128 or 256, any group of query heads; bases and outer
  *    strides of f16 tensors multiples of 16 bytes, position strides of keys and

@@ -63,7 +63,8 @@ constexpr int kReadAhead = 4;       // LDS operand reads in flight ahead of the 
 constexpr int kSchedMfma = 0x008, kSchedDsRead = 0x100;
 
 // A sequence as the plan sees it: its row tiles, the key tiles of the first and of the
-// last of them, and the position of its first row (negative: more rows than keys).
+// last of them, and the position of its first row (negative: more rows than keys; the
+// most that the table can name where it is further).
 struct Rows {
   uint32_t tiles, least, most;
   int32_t first;
@@ -71,14 +72,19 @@ struct Rows {
 
 // Key tiles of the row tiles of one sequence. Under the causal mask they grow from tile
 // to tile, else all are the same.
-template <int BN>
+template <int BN, bool PAGED>
 struct Tiles {
   Divisor group;
   uint32_t causal;
-  // Keys that the last row of tile i sees, of `tokens` tokens.
+  uint32_t cap;  // keys that the table can name (PAGED)
+  // Key tiles of a row tile whose last row is of token `last`.
+  __device__ __forceinline__ uint32_t keys(int32_t first, uint32_t last) const {
+    const int32_t seen = first + (int32_t)(PAGED ? min(last + 1, cap - (uint32_t)first) : last + 1);
+    return ((uint32_t)max(0, seen) + BN - 1) / BN;
+  }
+  // Key tiles of tile i, of `tokens` tokens.
   __device__ __forceinline__ uint32_t of(int32_t first, uint32_t tokens, uint32_t i) const {
-    const uint32_t last = causal != 0 ? min(tokens - 1, divide((i + 1) * BM - 1, group)) : tokens - 1;
-    return ((uint32_t)max(0, first + (int32_t)last + 1) + BN - 1) / BN;
+    return keys(first, causal != 0 ? min(tokens - 1, divide((i + 1) * BM - 1, group)) : tokens - 1);
   }
   __device__ __forceinline__ Rows sequence(int32_t first, uint32_t tokens) const {
     const uint32_t n = (tokens * group.value + BM - 1) / BM;
@@ -92,9 +98,7 @@ struct Tiles {
   }
   // Key tiles of tile i.
   __device__ __forceinline__ uint32_t at(Rows r, uint32_t i) const {
-    if (causal == 0 || i + 1 >= r.tiles) return r.most;
-    const int32_t last = (int32_t)divide((i + 1) * BM - 1, group);
-    return ((uint32_t)max(0, r.first + last + 1) + BN - 1) / BN;
+    return causal == 0 || i + 1 >= r.tiles ? r.most : keys(r.first, divide((i + 1) * BM - 1, group));
   }
 };
 
@@ -106,10 +110,9 @@ struct Piece {
 
 // The piece of `rank` (of one KV head), the same in every wave that asks. `share`: the
 // workgroups that the chip runs at once for one KV head.
-template <int BN>
-__device__ __forceinline__ bool plan_piece(const PackedParams &p, uint32_t rank, const Rows *s_rows,
+template <int BN, bool PAGED>
+__device__ __forceinline__ bool plan_piece(const PackedParams &p, const Tiles<BN, PAGED> &t, uint32_t rank, const Rows *s_rows,
                                            uint32_t *s_before, int lane, Piece *out) {
-  const Tiles<BN> t{p.group, p.causal};
   // The first 64 sequences stay in registers.
   const uint32_t own = min((uint32_t)lane, p.batch - 1);
   const bool is_own = (uint32_t)lane < p.batch;
@@ -265,32 +268,35 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     kvh = k - rest * per + (whole ? blockIdx.x % 8 * per : 0);
   }
   // The sequences' rows and first positions (every wave writes all of them, and reads back
-  // what it wrote itself), and the piece of this rank.
+  // what it wrote itself), and the piece of this rank. Positions past the table have no keys.
+  const uint32_t cap = PAGED ? p.kv.table_width << p.kv.page_shift : 0;
+  const Tiles<BN, PAGED> row_tiles{p.group, p.causal, cap};
   for (uint32_t c0 = 0; c0 < p.batch; c0 += 64) {
     const uint32_t bb = c0 + lane;
     if (bb >= p.batch) continue;
     const RowRange r = sequence_rows(p.row_starts, bb, p.rows);
     const uint32_t tokens = r.end - r.begin;
-    s_rows[bb] = Tiles<BN>{p.group, p.causal}.sequence(PAGED ? (int32_t)paged_length(p.kv, bb) - (int32_t)tokens : 0, tokens);
+    s_rows[bb] = row_tiles.sequence(PAGED ? (int32_t)min((int64_t)p.kv.lengths[bb] - tokens, (int64_t)cap) : 0, tokens);
   }
   Piece pc;
-  if (!plan_piece<BN>(p, rest, s_rows, s_before, lane, &pc)) return;
+  if (!plan_piece(p, row_tiles, rest, s_rows, s_before, lane, &pc)) return;
   const uint32_t b = __builtin_amdgcn_readfirstlane(pc.b), tile = __builtin_amdgcn_readfirstlane(pc.tile);
   const uint32_t t_begin = __builtin_amdgcn_readfirstlane(pc.begin), t_end = __builtin_amdgcn_readfirstlane(pc.end);
   const RowRange range = sequence_rows(p.row_starts, b, p.rows);
   const uint32_t tokens = range.end - range.begin;
   const uint32_t L = PAGED ? paged_length(p.kv, b) : tokens;
-  const int64_t off = (int64_t)L - tokens;  // position of the first row (negative: more rows than keys)
+  // Position of the first row (negative: more rows than keys).
+  const int64_t off = PAGED ? (int64_t)p.kv.lengths[b] - tokens : 0;
 
   const uint32_t row0 = tile * BM, my_row = row0 + wave * 32 + n;
   const uint32_t my_t = divide(my_row, p.group), my_g = my_row - my_t * G;
   const bool row_ok = my_t < tokens;
   const uint32_t t_first = divide(row0, p.group), t_last = min(tokens - 1, divide(row0 + BM - 1, p.group));
-  const uint32_t kmax = p.causal != 0 ? (uint32_t)max((int64_t)0, off + t_last + 1) : L;  // at most L
+  const uint32_t kmax = p.causal != 0 ? (uint32_t)max((int64_t)0, min(off + t_last + 1, (int64_t)L)) : L;
   const bool active = row0 + wave * 32 < tokens * G;  // whether this wave has rows
   // Last key that this lane's row sees, and that the tile's first row does.
-  const int64_t lim = p.causal != 0 ? off + min(my_t, tokens - 1) : (int64_t)L - 1;
-  const int64_t full_lim = p.causal != 0 ? off + t_first : (int64_t)L - 1;
+  const int64_t lim = p.causal != 0 ? min(off + min(my_t, tokens - 1), (int64_t)L - 1) : (int64_t)L - 1;
+  const int64_t full_lim = p.causal != 0 ? min(off + t_first, (int64_t)L - 1) : (int64_t)L - 1;
 
   // Q^T as the B operand: lane (h, n) holds Q[row n][16 c + 8 h .. + 8].
   h8_t qop[DC];

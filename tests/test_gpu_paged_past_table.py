@@ -5,7 +5,10 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from test_gpu_paged import Cache, append, hold, rotated, rows_for, starts_of
+from mi_attn import U32, AttentionConfig
+from helpers import f16
+from test_gpu_paged import (NOWHERE, Cache, append, attend, hold, paged, rotated, rows_for,
+                            starts_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +51,53 @@ def test_append_one_row_past_the_table(ctx):
     want = cache.value.copy()
     want[cache.table[1, 1], 15] = x[2][1].view(np.uint16)
     assert np.array_equal(cache.download(1), want)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("hq,hkv,d,size", [(4, 2, 128, 16), (5, 1, 64, 32), (3, 1, 256, 16), (4, 4, 32, 64)])
+def test_paged_rows_past_the_table(ctx, hq, hkv, d, size, causal):
+    """A row sees the keys up to its position that the table can name."""
+    rng = np.random.default_rng(d + size)
+    width = 1280 // size
+    full = width * size
+    cache = Cache(ctx, rng, [full, full, full, full, 40], width, size, hkv, d)
+    lengths = np.array([full + 5, full + 1000, NOWHERE, full, 40], np.int64)
+    counts = [70, 3, 40, 20, 60]  # of the last, 20 rows have no position
+    ctx.upload(cache.device_lengths, lengths.astype(np.uint32))
+    starts = starts_of(counts)
+    q = rng.standard_normal((int(starts[-1]), hq, d)).astype(np.float16)
+    got = paged(ctx, cache, q, starts, hq, causal)
+    for i, n in enumerate(counts):
+        a, e = starts[i], starts[i + 1]
+        k, v = cache.rows[i]
+        seen = [np.arange(max(0, min(len(k), lengths[i] - n + t + 1 if causal else lengths[i]))) for t in range(n)]
+        hold(got[a:e], *attend(q[a:e].astype(np.float64), k, v, seen, True), f"sequence {i}")
+
+
+def test_a_sequence_that_outgrows_its_table(ctx):
+    """Appended and read token by token past the end: the stored keys stay, and are all seen."""
+    rng = np.random.default_rng(2)
+    hq, hkv, d, size = 4, 2, 128, 16
+    cache = Cache(ctx, rng, [30], 2, size, hkv, d)
+    held = [[r] for r in cache.rows[0]]
+    cfg = AttentionConfig(hq, hkv, d)
+    for length in range(31, 37):
+        ctx.upload(cache.device_lengths, np.array([length], np.uint32))
+        x, weights = rows_for(rng, 1, hq, hkv, d)
+        q = append(ctx, cache, x, None, weights)
+        if length <= 32:
+            page = cache.table[0, (length - 1) // size], (length - 1) % size
+            held[0].append(cache.download(0)[page][None].view(np.float16))
+            held[1].append(x[2])
+        k, v = (np.concatenate(h) for h in held)
+        assert len(k) == min(length, 32)
+        out = ctx.empty((1, hq, d))
+        batch = ctx.begin_batch()
+        batch.attention_paged(ctx.tensor(q), cache.key_pages, cache.value_pages, cache.device_table, cache.device_lengths,
+                              ctx.tensor(starts_of([1]), U32), cfg, out=out)
+        one = batch.attention_decode_paged(ctx.tensor(q), cache.key_pages, cache.value_pages, cache.device_table,
+                                           cache.device_lengths, cfg)
+        batch.finish()
+        q64 = f16(q).astype(np.float64)
+        hold(ctx.download(out), *attend(q64, k, v, [np.arange(len(k))], True))
+        hold(ctx.download(one), *attend(q64, k, v, [np.arange(len(k))], False))
