@@ -427,6 +427,10 @@ mi_status mi_decode_step_attention(mi_batch *batch, const mi_tensor *q,
  *    strides of f16 tensors multiples of 16 bytes, position strides of keys and
  *    values not negative, a page (or 64 packed rows) of them within 2 GiB.
  *    config->query_offset (and the transform's offset) are ignored. Nothing is launched for N = 0 or B = 0.
+ *  - Workspace, from the batch's arena: packed and paged attention take up to
+ *    72 MiB for the partial results of row tiles whose keys several workgroups
+ *    share (256 CUs), less where few rows or keys bound it, and none below 16
+ *    tiles of 64 keys (32 at head_dim 256) or past 512 KV heads (256).
  *  - Tables, lengths and row offsets are read when the call runs on the GPU: a
  *    captured call reads what they hold at each replay. Outputs must not overlap
  *    inputs, except the transform's q_out, which may be q itself. */

@@ -28,6 +28,7 @@
 // being 1.34), by the bytes of K and V for a few rows on a long cache, and for short prompts
 // by what every row tile needs once: its place in the plan (2.5 us), Q and the first tile
 // (3 us) and the output (1.5 us), beside two such workgroups per CU.
+#include <algorithm>
 #include <type_traits>
 
 #include "paged_tile.hpp"
@@ -881,6 +882,12 @@ hipError_t launch_d(const PackedParams &p, const Launch &l) {
 
 uint32_t packed_workgroups(uint32_t compute_units, uint32_t head_dim) {
   return (head_dim == 256 ? 1 : 2) * (compute_units > 1 ? compute_units : 1);
+}
+
+uint64_t packed_pieces(uint64_t keys, uint64_t row_tiles, uint32_t head_dim) {
+  const uint64_t tiles = (keys + tile_keys(head_dim) - 1) / tile_keys(head_dim);
+  if (tiles < 2 * kLeastPiece) return 0;
+  return row_tiles * std::min<uint64_t>(kMostPieces, (tiles + kLeastPiece - 1) / kLeastPiece);
 }
 
 uint64_t packed_row_tiles(uint64_t rows, uint32_t batch, uint32_t group) {

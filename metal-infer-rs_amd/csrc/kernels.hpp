@@ -437,6 +437,8 @@ constexpr uint64_t packed_partial_floats(uint64_t pieces, uint64_t kv_heads, uin
 }
 uint32_t packed_workgroups(uint32_t compute_units, uint32_t head_dim);
 hipError_t launch_packed(const PackedParams &p, uint32_t head_dim, const Launch &l);
+// Most pieces per KV head that row tiles over at most `keys` keys are cut into (0: none is cut).
+uint64_t packed_pieces(uint64_t keys, uint64_t row_tiles, uint32_t head_dim);
 // Most row tiles of a KV head: every sequence may have a partial one.
 uint64_t packed_row_tiles(uint64_t rows, uint32_t batch, uint32_t group);
 // Head dimensions of the kernels over packed rows and pages.

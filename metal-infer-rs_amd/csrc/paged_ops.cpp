@@ -225,10 +225,15 @@ mi_status packed(mi_batch *batch, const mi_tensor *q, const mi_tensor *key, cons
     return fail(MI_ERR_SHAPE, "attention grid exceeds the launch limits");
   if ((st = check_batch(batch)) != MI_OK || q->shape[0] == 0 || sequences == 0) return st;
   p.row_tiles = (uint32_t)tiles;
-  // Twice the workgroups that run at once: an even share each, and a last piece per tile.
+  // Twice the workgroups that run at once: an even share each, and a last piece per tile;
+  // no more than the call's rows and keys can be cut into, and none where the KV heads alone
+  // fill the chip.
   Context *ctx = batch->ctx;
-  p.share = std::max(1u, kernels::packed_workgroups(ctx->compute_units, config->head_dim) / p.kv_heads);
-  p.max_pieces = (uint64_t)4 * p.share * p.kv_heads <= ctx->split_counter_count ? 2 * p.share : 0;
+  const uint32_t workgroups = kernels::packed_workgroups(ctx->compute_units, config->head_dim);
+  p.share = std::max(1u, workgroups / p.kv_heads);
+  const uint64_t keys = paged ? (uint64_t)p.kv.table_width << p.kv.page_shift : p.rows;
+  p.max_pieces = (uint32_t)std::min<uint64_t>(2 * p.share, kernels::packed_pieces(keys, tiles, config->head_dim));
+  if (p.kv_heads > workgroups || (uint64_t)2 * p.max_pieces * p.kv_heads > ctx->split_counter_count) p.max_pieces = 0;
   p.counters = ctx->split_counters;
   p.counter_stride = kernels::counter_stride((uint64_t)2 * p.max_pieces * p.kv_heads, ctx->split_counter_count);
   void *scratch = nullptr;
