@@ -667,14 +667,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_packed_kernel(cons
     // NaN, where the weight itself leaves the infinity. Where a row with a finite sum has a
     // value that is not finite, or a masked tile's were taken out, the workgroup looks at
     // the values of its keys again: a column's infinities and NaN decide it.
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // one chain of additions would take 0.2 us
+    float most = 0.0f;  // NaN if a value is
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sum[r & 3] = fmaf(o[dt][r], 0.0f, sum[r & 3]);
-    if (__any(sum[0] + sum[1] + sum[2] + sum[3] != 0.0f && l_total > 0.0f)) s_bad = 1;
+      for (int r = 0; r < 16; r += 2)
+        most = __builtin_elementwise_maximum(__builtin_elementwise_maximum(fabsf(o[dt][r]), fabsf(o[dt][r + 1])), most);
+    if (__any(!(most <= __FLT_MAX__) && l_total > 0.0f)) s_bad = 1;
     __syncthreads();  // also: every wave is past its last LDS operand read
-    if (s_bad != 0) {
+    if (__builtin_expect(s_bad != 0, 0)) {
       // The first keys of each column that hold an infinity or NaN, and a negative one or NaN.
       uint32_t *first = reinterpret_cast<uint32_t *>(k_lds_a);
       for (uint32_t i = tid; i < 2 * D; i += 256) first[i] = ~0u;
