@@ -229,7 +229,9 @@ def _batch():
 
 
 def _views(x):
-    """The tensors of a state as the framework's descriptors, which a program makes once."""
+    """The tensors of a state as the framework's descriptors, which a program makes once: the
+    state's tensors may be filled anew between passes but not replaced, and are held here, as a
+    descriptor does not keep its memory alive."""
     if _program["context"] is None:
         sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "metal-infer-rs_amd"))
     import mi_attn
@@ -246,6 +248,7 @@ def _views(x):
     names = ("q", "k", "v", "out", "table", "lengths", "row_starts", "key_pages", "value_pages")
     w = {k: view(x.get(k)) for k in names}
     w["q_weight"], w["k_weight"] = (view(t) for t in x.get("weights") or (None, None))
+    w["held"] = [x.get(k) for k in (*names, "weights")]
     hkv = (x["k"] if x["op"] in ("append", "packed") else x["key_pages"]).shape[-2]
     w["attention"] = mi_attn.AttentionConfig(x["q"].shape[1], hkv, x["q"].shape[2], True, 0)
     w["rope"] = mi_attn.QkNormRopeCacheConfig(0, THETA, EPS)
@@ -253,6 +256,8 @@ def _views(x):
 
 
 def _own(x):
+    """Enqueues on the context's stream, which torch's streams do not wait for: the caller waits
+    for the device before it reads the outputs, fills the inputs anew or drops the state."""
     if "views" not in x:
         x["views"] = _views(x)
     w, batch = x["views"], _batch()
