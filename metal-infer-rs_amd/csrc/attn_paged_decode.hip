@@ -34,8 +34,7 @@ using namespace mi::dev;
 constexpr int kWaves = kPagedWaves;
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
-// Workgroups per CU, by the registers of a wave.
-constexpr uint32_t per_cu(uint32_t) { return 2; }
+constexpr uint32_t kPerCu = 2;  // workgroups per CU, by the registers of a wave at head_dim 256
 // Fewest tiles of a workgroup's piece (one per wave) and of a wave's share.
 constexpr uint32_t kPiece = kWaves, kShare = 2;
 // Pieces may be longer than an even share by this many eighths; more than twice kJoin of a
@@ -73,10 +72,11 @@ __device__ __forceinline__ float sum32(float x) {
 }
 
 // How a launch divides its work, the same in every wave. With `piece` a position is a
-// piece of that many tiles of a unit, for a workgroup, else a tile, or with `whole` a unit,
-// for a wave; each takes `seg` of them. s_tiles[b] gets the sequences' tiles, s_pre[b] the positions of
-// all units before b's. Every wave computes all of it and reads back what it wrote
-// itself, so no barrier is needed (the waves write the same values).
+// piece of that many tiles of a unit, for a workgroup, which takes one at most; else it is
+// a tile, or with `whole` a unit, for a wave, which takes `seg` of them. s_tiles[b] gets the
+// sequences' tiles, s_pre[b] the positions of all units before b's. Every wave computes all
+// of it and reads back what it wrote itself, so no barrier is needed (the waves write the
+// same values).
 struct Share {
   uint32_t piece, seg, total;
   bool whole;
@@ -244,7 +244,7 @@ struct Unit {
 };
 
 template <int D>
-__global__ __launch_bounds__(kWaves * 64, per_cu(D)) void attn_decode_paged_kernel(const PagedDecodeParams p) {
+__global__ __launch_bounds__(kWaves * 64, kPerCu) void attn_decode_paged_kernel(const PagedDecodeParams p) {
   constexpr int WAVES = kWaves, KT = kDecodeTile, DC = D / 32, DB = D / 16;
   constexpr int CPR = D / 8, VL = KT * CPR / 64;  // 16-byte chunks per V row, 1 KB V loads per tile
   constexpr int THREADS = WAVES * 64, STAGE = KT * D, GM = kDecodeRows;
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(kWaves * 64, per_cu(D)) void attn_decode_paged_kern
   // Of a CU's two workgroups the older one's waves are served first and would end a fifth
   // earlier, leaving the other half of the loads to the tail. The younger's waves go first for
   // the first half of their tiles (32 sequences of 1024 to 8192 keys: 112 -> 108.5 us).
-  uint32_t ahead = blockIdx.x >= gridDim.x / 2 ? (together ? (sh.piece + WAVES - 1) / WAVES : 1) * sh.seg / 2 : 0;
+  uint32_t ahead = blockIdx.x >= gridDim.x / 2 ? (together ? (sh.piece + WAVES - 1) / WAVES : sh.seg) / 2 : 0;
   if (ahead != 0) __builtin_amdgcn_s_setprio(1);
   while (pos < end) {
     b = __builtin_amdgcn_readfirstlane(b);
@@ -474,7 +474,6 @@ __global__ __launch_bounds__(kWaves * 64, per_cu(D)) void attn_decode_paged_kern
     uint16_t *out = e->out + (int64_t)b * e->o_seq + (int64_t)h0 * o_head;
     float *partial = e->partial + (size_t)slot * (e->chunk * ROW);
     const Unit unit{b, j, slot - piece, pieces};
-    if (together) __syncthreads();
     // The wave's rows through its stage, so that a store's lanes are neighbours.
     float *rows = reinterpret_cast<float *>(stage);  // [GM][D]
     if ((uint32_t)col < GC) {
@@ -529,12 +528,10 @@ __global__ __launch_bounds__(kWaves * 64, per_cu(D)) void attn_decode_paged_kern
           if (d == 0) store_partial2(partial + g * ROW, M, L);
         }
       }
-      // A workgroup has several pieces in turn only if they are whole units.
       if (pieces > 1) {
         s_unit[0][0] = unit;
         split = 1;
       }
-      __syncthreads();  // the next piece's loads overwrite the stages
     }
     pos += together || sh.whole ? 1 : t1 - t0;
     if (pos < end && pos >= s_pre[b + 1]) b = sequence_at(pos);
@@ -590,8 +587,8 @@ hipError_t launch_d(const PagedDecodeParams &p, const Launch &l) {
 
 }  // namespace
 
-uint32_t paged_decode_workgroups(uint32_t compute_units, uint32_t head_dim) {
-  return per_cu(head_dim) * (compute_units > 1 ? compute_units : 1);
+uint32_t paged_decode_workgroups(uint32_t compute_units) {
+  return kPerCu * (compute_units > 1 ? compute_units : 1);
 }
 
 hipError_t launch_paged_decode(const PagedDecodeParams &p, uint32_t head_dim, const Launch &l) {

@@ -376,7 +376,7 @@ constexpr uint64_t paged_decode_partial_floats(uint64_t units, uint64_t workgrou
                                                uint32_t head_dim) {
   return (units + workgroups * kPagedWaves) * chunk * (head_dim + 2);
 }
-uint32_t paged_decode_workgroups(uint32_t compute_units, uint32_t head_dim);
+uint32_t paged_decode_workgroups(uint32_t compute_units);
 struct PagedDecodeParams {
   const uint16_t *q;
   int64_t q_seq, q_head;
@@ -393,8 +393,6 @@ struct PagedDecodeParams {
 };
 hipError_t launch_paged_decode(const PagedDecodeParams &p, uint32_t head_dim, const Launch &l);
 
-// Packed query rows [N, Hq, D] of `batch` sequences over their own packed rows of K and
-// V (kv.table null: kv.k_pos and v_pos are row strides), or over their pages.
 // Division of numbers below 2^31 by a known one, in two multiplications instead of some 25
 // instructions: with 2^l >= d, magic = floor(2^(31 + l) / d) + 1 exceeds the quotient by less
 // than 2^l / d, so x magic / 2^(31 + l) exceeds x / d by less than 2^-l <= 1 / d.
@@ -407,6 +405,8 @@ inline Divisor divisor(uint32_t d) {
   return {(uint32_t)((1ull << (31 + l)) / d + 1), 31 + l, d};
 }
 
+// Packed query rows [N, Hq, D] of `batch` sequences over their own packed rows of K and
+// V (kv.table null: kv.k_pos and v_pos are row strides), or over their pages.
 struct PackedParams {
   const uint16_t *q;
   int64_t q_tok, q_head;

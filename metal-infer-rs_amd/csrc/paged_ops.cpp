@@ -154,7 +154,7 @@ mi_status decode_paged(mi_batch *batch, const mi_tensor *q, const mi_tensor *key
   Context *ctx = batch->ctx;
   const uint32_t step = (uint32_t)std::min<uint64_t>(
       {kernels::kPagedMaxBatch, kernels::kPagedMaxUnits / upb, (kRows31 - 1) / (upb * most_tiles), p.batch});
-  p.workgroups = kernels::paged_decode_workgroups(ctx->compute_units, config->head_dim);
+  p.workgroups = kernels::paged_decode_workgroups(ctx->compute_units);
   if (p.workgroups + kernels::kPagedMaxUnits > ctx->split_counter_count)
     return fail(MI_ERR_RESOURCE, "too few split counters");
   p.step_counters = ctx->split_counters;
