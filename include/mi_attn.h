@@ -427,6 +427,10 @@ mi_status mi_decode_step_attention(mi_batch *batch, const mi_tensor *q,
  *    strides of f16 tensors multiples of 16 bytes, position strides of keys and
  *    values not negative, a page (or 64 packed rows) of them within 2 GiB.
  *    config->query_offset (and the transform's offset) are ignored. Nothing is launched for N = 0 or B = 0.
+ *  - Sums, maxima and softmax statistics are f32. Packed and paged attention
+ *    round the weights to f16 for the products with V, as the flash prefill does
+ *    (2.3e-4 to 2.9e-4 relative error against 64 bits with the output's own
+ *    rounding, which alone is 2.0e-4); the decode keeps 22 bits of them.
  *  - Workspace, from the batch's arena: packed and paged attention take up to
  *    72 MiB for the partial results of row tiles whose keys several workgroups
  *    share (256 CUs), less where few rows or keys bound it, and none below 16

@@ -51,7 +51,9 @@ constexpr float kBias = 8.0f;
 // Fewest key tiles of a piece of a cut row tile, and most pieces: a join costs as much as
 // some tiles (64 rows of 64 heads on 4000 keys: 32 us with at least 8, 42 us with 4), and the
 // time of many pieces' joins grows with them (32 rows of 32 heads on 16384 keys: 41, 38 and
-// 49 us with up to 16, 32 and 64; 272 us uncut).
+// 49 us with up to 16, 32 and 64; 272 us uncut). Both, and kOneJoin and join_size below, were
+// measured at head_dim 128; at 256 the same numbers stand, of tiles half as long and partials
+// twice as large.
 constexpr uint32_t kLeastPiece = 8, kMostPieces = 32;
 // More pieces than kOneJoin are joined a few at a time by several workgroups, and then those
 // joins: about the square root of their number. (64 rows of 64 heads on 4000 keys, 16 pieces
