@@ -92,3 +92,16 @@ def test_paged_scores_that_grow_from_piece_to_piece(ctx, d, total):
     toward(q, cache.rows[0][0], np.arange(keys), total * (np.arange(keys) // 64) / 94)
     stored(cache)
     hold(paged(ctx, cache, q, starts, 4), *paged_want(cache, q, starts, True))
+
+
+def test_row_starts_that_overlap_leave_nothing_behind(ctx):
+    """More row tiles, and more pieces of them, than the rows can have by themselves: the rows behind
+    stay as they are, and the call after it has its own results."""
+    rng = np.random.default_rng(5)
+    d, n, keys = 64, 1280, 20000
+    cache = Cache(ctx, rng, [keys, 40, keys, 40, keys], keys // 16, 16, 1, d)
+    q = rng.standard_normal((n + 2, 1, d)).astype(np.float16)
+    got = paged(ctx, cache, q, np.array([0, n, 0, n, 0, n], np.uint32), 1)
+    assert (got[n:] == 0x1234).all() and np.isfinite(got[:n].view(np.float16)).all()
+    starts = starts_of([2, 0, 1, 1, 1])
+    hold(paged(ctx, cache, q[:5], starts, 1), *paged_want(cache, q[:5], starts, True))
