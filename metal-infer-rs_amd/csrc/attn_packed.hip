@@ -23,11 +23,16 @@
 //    first, then the whole tiles with most keys first. The pieces of a cut tile leave
 //    their max, sum and weighted values (f32), and the last of them to finish joins them
 //    in order.
+//  - A weight of 0 (a masked key, or one below f16's range) times a value that is not finite
+//    is NaN: masked tiles' such values are taken out, and where they, or a NaN in a row with a
+//    finite sum, are found, the workgroup looks through its keys' values once more after the
+//    last tile and lets each column's infinities and NaN decide it.
 // Bound by the matrix instructions with the exponentials beside them for long prompts (two
-// of 4000 to 6000 rows, 32 heads on 8 of 128: 415 us, 1.0 PFLOP/s, a large f16 product's rate
-// being 1.34), by the bytes of K and V for a few rows on a long cache, and for short prompts
-// by what every row tile needs once: its place in the plan (2.5 us), Q and the first tile
-// (3 us) and the output (1.5 us), beside two such workgroups per CU.
+// of 4000 to 6000 rows, 32 heads on 8 of 128: 414 to 434 us on several cards, 0.96 to 1.0
+// PFLOP/s, a large f16 product's rate being 1.34), by the bytes of K and V for a few rows on a
+// long cache, and for short prompts by what every row tile needs once: its place in the plan
+// (2.5 us), Q and the first tile (3 us) and the output (1.5 us), beside two such workgroups
+// per CU.
 #include <algorithm>
 #include <type_traits>
 
